@@ -454,6 +454,37 @@ SOLID_API int solid_gpu_peer_sum_float(int world, int rank, void *const *buffers
                                        int *status, cudaStream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* The 8-bit linear layer: norm, conversion to 8 bits with scales, product.   */
+/* No counterpart in the reference.  dtype is SD_HALF, SD_FLOAT or SD_DOUBLE.  */
+/* Sums and norms are kept in 32 bits (double: 64); results are rounded once,  */
+/* to nearest even.  Matrices are [n, rows] with strides of their own; those   */
+/* marked optional may be NULL.  An output may stand in place of an input with  */
+/* the same strides; other overlaps are not allowed.                            */
+/*   rms_norm           h = x + residual (optional), y = h * w / sqrt(mean(h^2) + eps) along dimension 0;              */
+/*                      w: n elements of the same type (optional: ones); h is also stored when given                   */
+/*   rms_norm_quantize  the same, y as codes with one scale for 128 elements of a row (y->block 1)                     */
+/*   rms_norm_grad      from dy and h: dh = r (dy w) - h r^3 mean(dy w h) (+ dres, optional), r = 1 / sqrt(mean(h^2)   */
+/*                      + eps), and dweight = sum over the rows of dy h r: n elements of the work type (half: float),  */
+/*                      optional.  buffer: device memory of rms_norm_grad_buffer_size bytes                            */
+/*   block_quantize     codes and scales of x: scale = max(largest magnitude / largest code, 2^-126) over 128 elements  */
+/*                      of dimension 0 by y->block rows, code = x / scale rounded to nearest even (in 32 bits)         */
+/*   block_gemm         c[m, n] = sum over k of a[k, m] * b[k, n], a of size [K, M], b [K, N], c half or float [M, N]  */
+SOLID_API int solid_gpu_rms_norm(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x, const solid_gpu_matrix *residual,
+                                 const void *weight, double eps, const solid_gpu_matrix *h, const solid_gpu_matrix *y,
+                                 cudaStream_t stream);
+SOLID_API int solid_gpu_rms_norm_quantize(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x, const solid_gpu_matrix *residual,
+                                          const void *weight, double eps, const solid_gpu_matrix *h, const solid_gpu_blocks *y,
+                                          cudaStream_t stream);
+SOLID_API int solid_gpu_rms_norm_grad_buffer_size(int dtype, size_t n, size_t rows, int device, size_t *size);
+SOLID_API int solid_gpu_rms_norm_grad(int dtype, size_t n, size_t rows, const solid_gpu_matrix *dy, const solid_gpu_matrix *h,
+                                      const void *weight, double eps, const solid_gpu_matrix *dres, const solid_gpu_matrix *dh,
+                                      void *dweight, void *buffer, cudaStream_t stream);
+SOLID_API int solid_gpu_block_quantize(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x, const solid_gpu_blocks *y,
+                                       cudaStream_t stream);
+SOLID_API int solid_gpu_block_gemm(int ctype, size_t M, size_t N, size_t K, const solid_gpu_blocks *a, const solid_gpu_blocks *b,
+                                   const solid_gpu_matrix *c, cudaStream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Axis sum of float tensors for callers that may not allocate.  It has no    */
 /* counterpart in the reference.  Some callers cannot obtain device memory at  */
 /* the point where they reduce: a callback or destructor that runs while an    */

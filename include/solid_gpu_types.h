@@ -172,4 +172,24 @@ typedef struct {
    int              byteswapped;  /* 0 or 1 */
 } solid_gpu_operand;
 
+/* A matrix of the row operators: element (i, row) at ptr + i * stride0 + row * stride1 (bytes).  Dimension 0 is the   */
+/* one that a norm or a block of 128 runs along.                                                                        */
+typedef struct {
+   void     *ptr;
+   ptrdiff_t stride0, stride1;
+} solid_gpu_matrix;
+
+/* A matrix of 8-bit floating-point codes with scales: code (i, row) at codes + i + row * ld, its scale at              */
+/* scales + (row / block) * scale_stride0 + (i / 128) * scale_stride1 (strides in bytes); it stands for code * scale.   */
+typedef struct {
+   void     *codes;
+   ptrdiff_t ld;
+   float    *scales;
+   ptrdiff_t scale_stride0, scale_stride1;
+   int       block;         /* rows that share a scale: 1 or 128   */
+   int       format;        /* SOLID_GPU_E4M3 or SOLID_GPU_E5M2    */
+} solid_gpu_blocks;
+#define SOLID_GPU_E4M3 0
+#define SOLID_GPU_E5M2 1
+
 #endif

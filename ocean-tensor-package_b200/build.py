@@ -14,6 +14,7 @@ import argparse
 import concurrent.futures as cf
 import hashlib
 import os
+import re
 import subprocess
 import sys
 import time
@@ -32,7 +33,8 @@ TYPES = {"bool": 0, "uint8": 1, "uint16": 1, "uint32": 1, "uint64": 1,
          "int8": 2, "int16": 2, "int32": 2, "int64": 2,
          "half": 3, "float": 3, "double": 3, "chalf": 4, "cfloat": 4, "cdouble": 4}
 PER_TYPE_UNITS = ["reduce", "copy", "unary", "binary", "fill", "steps"]     # slowest first
-SINGLE_UNITS = ["base", "luts", "reduce_plan", "fused", "noalloc", "index", "gemm", "peer"]
+SINGLE_UNITS = ["base", "luts", "reduce_plan", "fused", "noalloc", "index", "gemm", "peer",
+                "rms_norm", "block_quantize", "block_gemm"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O3", "-lineinfo",
               "--fmad=false",            # one rounding per operation, as the CPU oracle computes
@@ -48,10 +50,21 @@ def nvcc() -> str:
     return "nvcc"
 
 
-def _stamp() -> str:
+def _included(path: Path, seen: dict) -> dict:
+    """The unit's own headers, found by following its quoted includes: a header rebuilds the units that use it."""
+    for name in re.findall(r'^\s*#\s*include\s+"([^"]+)"', path.read_text(), re.M):
+        for folder in (CSRC, INCLUDE):
+            header = folder / name
+            if header.exists() and name not in seen:
+                seen[name] = header
+                _included(header, seen)
+    return seen
+
+
+def _stamp(src: Path) -> str:
     h = hashlib.sha256()
-    for path in sorted(list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list(INCLUDE.glob("*.h"))):
-        h.update(path.name.encode())
+    for name, path in sorted(_included(src, {}).items()):
+        h.update(name.encode())
         h.update(path.read_bytes())
     h.update(" ".join(NVCC_FLAGS).encode())
     return h.hexdigest()
@@ -68,9 +81,9 @@ def _jobs(types):
     return jobs
 
 
-def _compile(job, stamp, force):
+def _compile(job, force):
     src, obj, defs = job
-    key = hashlib.sha256((stamp + src.read_text() + " ".join(defs)).encode()).hexdigest()
+    key = hashlib.sha256((_stamp(src) + src.read_text() + " ".join(defs)).encode()).hexdigest()
     keyfile = obj.with_suffix(".key")
     if not force and obj.exists() and keyfile.exists() and keyfile.read_text() == key:
         return obj, 0.0, False
@@ -87,11 +100,10 @@ def build(jobs_n: int | None = None, force: bool = False, types=None, verbose: b
     types = list(types or TYPES)
     BUILD.mkdir(exist_ok=True)
     LIBDIR.mkdir(exist_ok=True)
-    stamp = _stamp()
     jobs = _jobs(types)
     objects, rebuilt = [], False
     with cf.ThreadPoolExecutor(max_workers=jobs_n or os.cpu_count() or 4) as pool:
-        futs = [pool.submit(_compile, j, stamp, force) for j in jobs]
+        futs = [pool.submit(_compile, j, force) for j in jobs]
         for f in futs:
             obj, secs, did = f.result()
             objects.append(obj)
@@ -108,7 +120,7 @@ def build(jobs_n: int | None = None, force: bool = False, types=None, verbose: b
         if verbose:
             print("[build] linked", LIB, flush=True)
     # the dispatch layer is host code only; it links against the Solid library beside it
-    obj, secs, did = _compile((CSRC / "ocean_gpu.cu", BUILD / "ocean_gpu.o", []), stamp, force)
+    obj, secs, did = _compile((CSRC / "ocean_gpu.cu", BUILD / "ocean_gpu.o", []), force)
     if did or rebuilt or not OCEAN_LIB.exists():
         cmd = [nvcc(), "-shared", "-o", str(OCEAN_LIB), str(obj), "-L%s" % LIBDIR, "-lsolid_core_gpu",
                "-Xlinker", "-rpath", "-Xlinker", "$ORIGIN", "-lcudart",

@@ -1,0 +1,454 @@
+// solid_gpu_block_gemm: product of two matrices of 8-bit floating-point codes with a scale for each 128 of the depth,
+//
+//   c[m, n] = sum over blocks kb of  sa[m, kb] sb[n, kb]  sum over k in kb of  a[k, m] b[k, n]
+//
+// The inner sum runs on the tensor cores into tensor memory (products of two codes are exact, sums have 32 bits); after
+// each block of 128 the epilogue's warps read it, apply both scales and add it to sums in registers.  While they do,
+// the tensor core works on the next block into the other half of tensor memory.
+//
+// Tiles of 128 x BN.  The 128 side lies on tensor memory's lanes, a thread of the epilogue each, so that its scale is one
+// register; the BN side lies on the columns, where a scale for 128 rows is one number a block as well, and a scale for
+// every row is a vector from shared memory.  Many tokens: tokens on the lanes, weights (128 x 128 scales) on the
+// columns, BN 256 or 128.  Few tokens: weights on the lanes, the tokens on 16 to 128 columns, and where the tiles do not
+// fill the GPU a cluster of blocks shares a tile, each with a part of the depth, and adds the parts up through
+// distributed shared memory in the order of the blocks.
+//
+// Operands whose codes are not on 16-byte boundaries take a plain kernel (shared-memory tiles, 32-bit arithmetic).
+#include <cuda.h>
+#include <mutex>
+#include "block8.cuh"
+#include "tcgen05.cuh"
+
+namespace sd {
+
+struct Side {                                             // one operand as a kernel sees it
+   const uint8_t *codes; int64_t ld;
+   const float *scale; int64_t s0, s1;                    // scale of (row block, depth block), strides in floats
+   int64_t rows; int shift, format;                       // shift: 0 or 7, rows that share a scale as a power of two
+};
+struct GemmArgs {
+   Side p, q;                                             // p on the lanes, q on the columns
+   int64_t K;
+   char *c; int64_t cp, cq;                               // element (row of p, row of q) at c + p * cp + q * cq
+   int half_out;
+};
+
+__device__ __forceinline__ float scale_at(const Side &s, int64_t row, int64_t kb)
+{
+   return row < s.rows ? __ldg(s.scale + (row >> s.shift) * s.s0 + kb * s.s1) : 0.0f;
+}
+__device__ __forceinline__ void store_c(const GemmArgs &a, int64_t p, int64_t q, float v)
+{
+   char *d = a.c + p * a.cp + q * a.cq;
+   if (a.half_out) *reinterpret_cast<__half *>(d) = __float2half_rn(v);
+   else            *reinterpret_cast<float *>(d) = v;
+}
+__device__ __forceinline__ float decode(uint8_t code, int format)
+{
+   uint32_t h;
+   if (format == B8_E4M3) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
+   else                   asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
+   return __half2float(__ushort_as_half((uint16_t)h));
+}
+
+// ---------------------------------------------------------------------------
+// any alignment: 64 x 64 tiles, four by four sums a thread
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) gemm_plain(const __grid_constant__ GemmArgs a)
+{
+   __shared__ float sp[32][65], sq[32][65];
+   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+   const int64_t ptiles = (a.p.rows + 63) / 64;
+   const int64_t p0 = blockIdx.x % ptiles * 64, q0 = blockIdx.x / ptiles * 64;
+   float acc[4][4] = {};
+   for (int64_t kb = 0; kb * B8_BLOCK < a.K; kb++) {
+      float sum[4][4] = {};
+      for (int k0 = 0; k0 < B8_BLOCK; k0 += 32) {
+         __syncthreads();
+#pragma unroll
+         for (int e = 0; e < 8; e++) {
+            const int r = (threadIdx.x >> 5) + 8 * e, k = threadIdx.x & 31;
+            const int64_t kk = kb * B8_BLOCK + k0 + k;
+            sp[k][r] = p0 + r < a.p.rows && kk < a.K ? decode(a.p.codes[(p0 + r) * a.p.ld + kk], a.p.format) : 0.0f;
+            sq[k][r] = q0 + r < a.q.rows && kk < a.K ? decode(a.q.codes[(q0 + r) * a.q.ld + kk], a.q.format) : 0.0f;
+         }
+         __syncthreads();
+#pragma unroll 4
+         for (int k = 0; k < 32; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+               for (int j = 0; j < 4; j++) sum[i][j] = fmaf(sp[k][tx + 16 * i], sq[k][ty + 16 * j], sum[i][j]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+         const float s = scale_at(a.p, p0 + tx + 16 * i, kb);
+#pragma unroll
+         for (int j = 0; j < 4; j++) acc[i][j] = fmaf(sum[i][j], s * scale_at(a.q, q0 + ty + 16 * j, kb), acc[i][j]);
+      }
+   }
+#pragma unroll
+   for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+         if (p0 + tx + 16 * i < a.p.rows && q0 + ty + 16 * j < a.q.rows) store_c(a, p0 + tx + 16 * i, q0 + ty + 16 * j, acc[i][j]);
+}
+
+// ---------------------------------------------------------------------------
+// tensor cores
+// ---------------------------------------------------------------------------
+constexpr int BM = 128;
+constexpr int TILE_P = BM * B8_BLOCK;                     // bytes of a stage's 128 rows
+
+template <int BN> struct Shape {
+   static constexpr int groups = BN > 128 ? 2 : 1;        // epilogue warpgroups, 128 columns at most each
+   static constexpr int columns = BN / groups;
+   static constexpr int threads = groups * 128 + 64;      // and a warp that loads, a warp that multiplies
+   static constexpr int stage = TILE_P + BN * B8_BLOCK;
+   static constexpr int resident = BN >= 128 ? 1 : 2;     // blocks an SM: one whose ring fills shared memory, or two
+   static constexpr int stages = BN == 256 ? 4 : BN == 128 ? 6 : BN == 64 ? 4 : BN == 32 ? 5 : 6;
+   static constexpr int tmem = 2 * BN < 32 ? 32 : 2 * BN;
+   static constexpr int scales = 2 * BN * 4;              // two blocks' scales of the columns
+   static constexpr int smem = 1024 + stages * stage + scales;
+};
+
+// COLVEC: a scale for every row of q (a vector over the columns); otherwise for 128 rows (one number).
+// SPLIT: a cluster shares the tile, block r takes the r-th part of the depth.
+template <int BN, bool COLVEC, bool SPLIT>
+__global__ void __launch_bounds__(Shape<BN>::threads, Shape<BN>::resident)
+gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ GemmArgs a,
+           int splits, int kblocks, int ptiles, int qtiles)
+{
+   using S = Shape<BN>;
+   constexpr int ST = S::stages, CW = S::columns;
+   extern __shared__ char raw[];
+   __shared__ alignas(8) uint64_t bars[2 * ST + 4];
+   __shared__ uint32_t tmem_base;
+   __shared__ int failed;
+   char *ring = raw + ((1024 - (tc::smem_u32(raw) & 1023)) & 1023);
+   float *colscale = (float *)(ring + ST * S::stage);     // [2][BN]
+   const uint32_t ring_u = tc::smem_u32(ring);
+   const uint32_t full = tc::smem_u32(bars), empty = full + 8 * ST, tfull = full + 16 * ST, tempty = tfull + 16;
+   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+   constexpr int EPI = S::groups * 4;                     // epilogue warps come first: warp w reads lanes 32 (w % 4)
+
+   if (threadIdx.x == 0) {
+      for (int s = 0; s < ST; s++) { tc::bar_init(full + 8 * s, 1); tc::bar_init(empty + 8 * s, 1); }
+      for (int b = 0; b < 2; b++) { tc::bar_init(tfull + 8 * b, 1); tc::bar_init(tempty + 8 * b, EPI); }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      failed = 0;
+   }
+   if (warp == EPI) tc::alloc(tc::smem_u32(&tmem_base), S::tmem);
+   tc::fence_before();
+   __syncthreads();
+   tc::fence_after();
+   const uint32_t tmem = *(volatile uint32_t *)&tmem_base;
+
+   const int ntiles = ptiles * qtiles;
+   const int rank = SPLIT ? (int)tc::cluster_rank() : 0;
+   const int first = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x, step = SPLIT ? ntiles : (int)gridDim.x;
+   const int kb0 = SPLIT ? (int)((long long)kblocks * rank / splits) : 0;
+   const int kb1 = SPLIT ? (int)((long long)kblocks * (rank + 1) / splits) : kblocks;
+   // Tiles in panels of 16 rows of tiles, so that blocks at work share both operands in the L2 cache
+   auto place = [&](int tile, int &tp, int &tq) {
+      const int panel = tile / (16 * qtiles), rest = tile - panel * 16 * qtiles;
+      const int height = min(16, ptiles - panel * 16);
+      tp = panel * 16 + rest % height; tq = rest / height;
+   };
+
+   if (warp == EPI && lane == 0) {                        // ---- loads
+      int it = 0; bool ok = true;
+      for (int tile = first; tile < ntiles && ok; tile += step) {
+         int tp, tq; place(tile, tp, tq);
+         for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int s = it % ST;
+            if (it >= ST && !tc::bar_wait(empty + 8 * s, (it / ST - 1) & 1)) { ok = false; break; }
+            const uint32_t dst = ring_u + s * S::stage;
+            tc::bar_expect(full + 8 * s, S::stage);
+            tc::load_box(dst, &map_p, full + 8 * s, kb * B8_BLOCK, tp * BM);
+            tc::load_box(dst + TILE_P, &map_q, full + 8 * s, kb * B8_BLOCK, tq * BN);
+         }
+      }
+      if (!ok) {                                          // the copies under way end before shared memory is given back
+         *(volatile int *)&failed = 1;
+         for (int k = max(0, it - ST); k < it; k++) tc::bar_wait(full + 8 * (k % ST), (k / ST) & 1);
+      }
+   } else if (warp == EPI + 1 && lane == 0) {             // ---- products
+      const uint32_t idesc = (1u << 4) | ((uint32_t)a.p.format << 7) | ((uint32_t)a.q.format << 10) | ((uint32_t)(BN / 8) << 17) | ((uint32_t)(BM / 16) << 24);
+      int it = 0; bool ok = true;
+      for (int tile = first; tile < ntiles && ok; tile += step)
+         for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int s = it % ST, b = it & 1;
+            if (it >= 2 && !tc::bar_wait(tempty + 8 * b, (it / 2 - 1) & 1)) { ok = false; break; }
+            if (!tc::bar_wait(full + 8 * s, (it / ST) & 1)) { ok = false; break; }
+            tc::fence_after();
+            const uint64_t dp = tc::tile_descriptor(ring_u + s * S::stage), dq = tc::tile_descriptor(ring_u + s * S::stage + TILE_P);
+#pragma unroll
+            for (int k = 0; k < 4; k++) tc::mma_f8(tmem + b * BN, dp + 2 * k, dq + 2 * k, idesc, k > 0);
+            tc::commit(empty + 8 * s);
+            tc::commit(tfull + 8 * b);
+         }
+      if (!ok) {
+         *(volatile int *)&failed = 1;
+         if (it > 0) tc::bar_wait(tfull + 8 * ((it - 1) & 1), ((it - 1) / 2) & 1);
+      }
+   } else if (warp < EPI) {                               // ---- scales and sums
+      const int group = warp >> 2, row = (warp & 3) * 32 + lane, col0 = group * CW;
+      const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + col0;
+      int it = 0; bool ok = true;
+      for (int tile = first; tile < ntiles; tile += step) {
+         int tp, tq; place(tile, tp, tq);
+         const int64_t p = (int64_t)tp * BM + row, q0 = (int64_t)tq * BN + col0;
+         const int64_t my_col = COLVEC ? q0 + row : q0;   // the column whose scale this thread fetches
+         const bool fetches = !COLVEC || row < CW;
+         uint64_t acc[CW / 2];
+#pragma unroll
+         for (int j = 0; j < CW / 2; j++) acc[j] = 0;
+         // scales are fetched two blocks ahead
+         float sp[3], sq[3];
+#pragma unroll
+         for (int d = 0; d < 2; d++) {
+            sp[d] = kb0 + d < kb1 ? scale_at(a.p, p, kb0 + d) : 0.0f;
+            sq[d] = kb0 + d < kb1 && fetches ? scale_at(a.q, my_col, kb0 + d) : 0.0f;
+         }
+         for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int b = it & 1;
+            sp[2] = kb + 2 < kb1 ? scale_at(a.p, p, kb + 2) : 0.0f;
+            sq[2] = kb + 2 < kb1 && fetches ? scale_at(a.q, my_col, kb + 2) : 0.0f;
+            const float *cs = colscale + b * BN + col0;
+            if (COLVEC) {
+               if (fetches) colscale[b * BN + col0 + row] = sq[0];
+               if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+               else            asm volatile("bar.sync 2, 128;" ::: "memory");
+            }
+            const float s0 = COLVEC ? sp[0] : sp[0] * sq[0];
+            const uint64_t s2 = tc::pair(__float_as_uint(s0), __float_as_uint(s0));
+            if (ok && !tc::bar_wait(tfull + 8 * b, (it / 2) & 1)) { ok = false; *(volatile int *)&failed = 1; }
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            tc::fence_after();
+            uint32_t v[2][16];
+            tc::ld16(from + b * BN, v[0]);
+#pragma unroll
+            for (int c = 0; c < CW / 16; c++) {
+               tc::ld_wait(v[c & 1]);
+               if (c + 1 < CW / 16) tc::ld16(from + b * BN + 16 * (c + 1), v[(c + 1) & 1]);
+               else {
+                  tc::fence_before();
+                  __syncwarp();
+                  if (lane == 0) tc::bar_arrive(tempty + 8 * b);
+               }
+#pragma unroll
+               for (int j = 0; j < 16; j += 4) {
+                  uint64_t x = tc::pair(v[c & 1][j], v[c & 1][j + 1]), y = tc::pair(v[c & 1][j + 2], v[c & 1][j + 3]);
+                  if (COLVEC) {
+                     const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(cs + 16 * c + j);
+                     x = tc::mul2(x, w.x); y = tc::mul2(y, w.y);
+                  }
+                  acc[8 * c + j / 2] = tc::fma2(x, s2, acc[8 * c + j / 2]);
+                  acc[8 * c + j / 2 + 1] = tc::fma2(y, s2, acc[8 * c + j / 2 + 1]);
+               }
+            }
+            sp[0] = sp[1]; sp[1] = sp[2]; sq[0] = sq[1]; sq[1] = sq[2];
+         }
+         if (!ok) {                                       // a wait ran out: no result is better than a wrong one
+            const uint64_t nan = 0x7FFFFFFF7FFFFFFFull;
+#pragma unroll
+            for (int j = 0; j < CW / 2; j++) acc[j] = nan;
+         }
+         if (SPLIT) {
+            // this block's part to shared memory, over the ring: all its copies have been consumed
+            float *part = (float *)ring;
+#pragma unroll
+            for (int j = 0; j < CW / 2; j++) {
+               part[(col0 + 2 * j) * BM + row] = tc::lo_of(acc[j]);
+               part[(col0 + 2 * j + 1) * BM + row] = tc::hi_of(acc[j]);
+            }
+         } else if (p < a.p.rows) {
+            const int64_t es = a.half_out ? 2 : 4;
+            char *d = a.c + p * a.cp + q0 * a.cq;
+            if (a.cq == es && ((uintptr_t)d & 15) == 0) {
+               // a thread's outputs lie side by side: 16 bytes at a time
+               if (a.half_out) {
+#pragma unroll
+                  for (int j = 0; j < CW / 2; j += 4) {
+                     uint32_t w[4];
+#pragma unroll
+                     for (int k = 0; k < 4; k++) {
+                        const __half2 h = __floats2half2_rn(tc::lo_of(acc[j + k]), tc::hi_of(acc[j + k]));
+                        w[k] = *reinterpret_cast<const uint32_t *>(&h);
+                     }
+                     if (q0 + 2 * j + 8 <= a.q.rows) *reinterpret_cast<uint4 *>(d + 4 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+                     else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) if (q0 + 2 * j + k < a.q.rows) reinterpret_cast<uint16_t *>(d)[2 * j + k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+                     }
+                  }
+               } else {
+#pragma unroll
+                  for (int j = 0; j < CW / 2; j += 2) {
+                     const float4 w = make_float4(tc::lo_of(acc[j]), tc::hi_of(acc[j]), tc::lo_of(acc[j + 1]), tc::hi_of(acc[j + 1]));
+                     if (q0 + 2 * j + 4 <= a.q.rows) *reinterpret_cast<float4 *>(d + 8 * j) = w;
+                     else {
+                        if (q0 + 2 * j < a.q.rows) reinterpret_cast<float *>(d)[2 * j] = w.x;
+                        if (q0 + 2 * j + 1 < a.q.rows) reinterpret_cast<float *>(d)[2 * j + 1] = w.y;
+                        if (q0 + 2 * j + 2 < a.q.rows) reinterpret_cast<float *>(d)[2 * j + 2] = w.z;
+                     }
+                  }
+               }
+            } else {
+#pragma unroll
+               for (int j = 0; j < CW / 2; j++) {
+                  if (q0 + 2 * j < a.q.rows) store_c(a, p, q0 + 2 * j, tc::lo_of(acc[j]));
+                  if (q0 + 2 * j + 1 < a.q.rows) store_c(a, p, q0 + 2 * j + 1, tc::hi_of(acc[j]));
+               }
+            }
+         }
+      }
+   }
+   __syncwarp();
+   __syncthreads();
+   if (SPLIT) {                                           // the blocks' parts, added in the order of the blocks
+      if (failed) for (int e = threadIdx.x; e < BN * BM; e += S::threads) ((float *)ring)[e] = __int_as_float(0x7FFFFFFF);
+      tc::cluster_sync();
+      int tp, tq; place(first, tp, tq);
+      const uint32_t part = tc::smem_u32(ring);
+      const int cols = min(BN, (int)(a.q.rows - (int64_t)tq * BN));
+      for (int e = rank * S::threads + threadIdx.x; e < cols * BM; e += splits * S::threads) {
+         float v = 0;
+         for (int r = 0; r < splits; r++) v += tc::peer_load(part + 4 * e, r);
+         const int64_t p = (int64_t)tp * BM + (e & (BM - 1)), q = (int64_t)tq * BN + (e >> 7);
+         if (p < a.p.rows) store_c(a, p, q, v);
+      }
+      tc::cluster_sync();
+   }
+   if (warp == EPI) tc::dealloc(tmem, S::tmem);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encoder()
+{
+   static EncodeTiled f = [] {
+      void *p = nullptr; cudaDriverEntryPointQueryResult found;
+      if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+          found != cudaDriverEntryPointSuccess) { cudaGetLastError(); p = nullptr; }
+      return (EncodeTiled)p;
+   }();
+   return f;
+}
+
+static int map_of(CUtensorMap *map, const Side &s, int64_t K, int box_rows)
+{
+   EncodeTiled f = encoder();
+   if (f == nullptr) SD_ERROR("block_gemm: the driver has no tensor maps");
+   const cuuint64_t dims[2] = { (cuuint64_t)K, (cuuint64_t)s.rows };
+   const cuuint64_t strides[1] = { (cuuint64_t)(s.rows == 1 ? (K + 15) / 16 * 16 : s.ld) };
+   const cuuint32_t box[2] = { B8_BLOCK, (cuuint32_t)box_rows }, ones[2] = { 1, 1 };
+   if (f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)s.codes, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      SD_ERROR("block_gemm: the driver refused a tensor map");
+   return 0;
+}
+
+template <int BN, bool COLVEC, bool SPLIT>
+static int launch_tiles(const GemmArgs &a, int splits, int sms, cudaStream_t stream)
+{
+   using S = Shape<BN>;
+   CUtensorMap map_p, map_q;
+   if (map_of(&map_p, a.p, a.K, BM) != 0 || map_of(&map_q, a.q, a.K, BN) != 0) return -1;
+   auto *kernel = gemm_tiles<BN, COLVEC, SPLIT>;
+   SD_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
+   const int64_t ptiles = (a.p.rows + BM - 1) / BM, qtiles = (a.q.rows + BN - 1) / BN;
+   const int kblocks = (int)((a.K + B8_BLOCK - 1) / B8_BLOCK);
+   cudaLaunchConfig_t cfg = {};
+   const int64_t room = (int64_t)sms * S::resident;
+   cfg.gridDim = dim3((unsigned)(SPLIT ? ptiles * qtiles * splits : std::min(ptiles * qtiles, room)));
+   cfg.blockDim = dim3(S::threads);
+   cfg.dynamicSmemBytes = S::smem;
+   cfg.stream = stream;
+   cudaLaunchAttribute attr[1];
+   if (SPLIT) {
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr; cfg.numAttrs = 1;
+   }
+   SD_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, a, splits, kblocks, (int)ptiles, (int)qtiles));
+   return 0;
+}
+
+template <int BN> static int launch_width(const GemmArgs &a, int splits, int sms, cudaStream_t stream)
+{
+   const bool vec = a.q.shift == 0;
+   if (splits > 1) return vec ? launch_tiles<BN, true, true>(a, splits, sms, stream) : launch_tiles<BN, false, true>(a, splits, sms, stream);
+   return vec ? launch_tiles<BN, true, false>(a, 1, sms, stream) : launch_tiles<BN, false, false>(a, 1, sms, stream);
+}
+
+static bool on_boundaries(const Side &s, int64_t K)
+{
+   return (uintptr_t)s.codes % 16 == 0 && (s.rows == 1 || (s.ld % 16 == 0 && s.ld >= K && s.ld < ((int64_t)1 << 39))) &&
+          s.rows < 0x7FFFFFFF - 256;
+}
+
+static int gemm(GemmArgs &a, cudaStream_t stream)
+{
+   DeviceInfo dev;
+   if (current_device_info(&dev) != 0) return -1;
+   if (a.K == 0 || a.K > 0x7FFFFF00 || !on_boundaries(a.p, a.K) || !on_boundaries(a.q, a.K)) {
+      const int64_t pt = (a.p.rows + 63) / 64, qt = (a.q.rows + 63) / 64, tiles = pt * qt;
+      if (pt > 0x7FFFFFFF / qt) SD_ERROR("block_gemm: matrix too large");
+      gemm_plain<<<(unsigned)tiles, 256, 0, stream>>>(a);
+      SD_LAUNCH_CHECK();
+      return 0;
+   }
+   // Few tokens: the wider matrix on the lanes, the narrow one on just enough columns.  Many: the matrix with scales for
+   // 128 rows on the columns, where they cost nothing.
+   const int64_t narrow = std::min(a.p.rows, a.q.rows);
+   const bool swap = narrow <= 128 ? a.q.rows > a.p.rows : (a.q.shift == 0 && a.p.shift == 7);
+   if (swap) { std::swap(a.p, a.q); std::swap(a.cp, a.cq); }
+   const int64_t ptiles = (a.p.rows + BM - 1) / BM;
+   int bn = 256;
+   if (a.q.rows <= 16) bn = 16; else if (a.q.rows <= 32) bn = 32; else if (a.q.rows <= 64) bn = 64; else if (a.q.rows <= 128) bn = 128;
+   else if (ptiles * ((a.q.rows + 255) / 256) < dev.sms) bn = 128;
+   const int64_t qtiles = (a.q.rows + bn - 1) / bn, tiles = ptiles * qtiles, kblocks = (a.K + B8_BLOCK - 1) / B8_BLOCK;
+   if (ptiles > 0x3FFFFFF / qtiles) SD_ERROR("block_gemm: matrix too large");
+   // A tile is shared by up to eight blocks (the portable size of a cluster) while there is room on the GPU and two
+   // depth blocks are left for each.
+   int splits = 1;
+   const int64_t room = (int64_t)dev.sms * (bn < 128 ? 2 : 1);
+   while (splits < 8 && tiles * splits * 2 <= room && kblocks >= 4 * splits) splits *= 2;
+   switch (bn) {
+      case 16:  return launch_width<16>(a, splits, dev.sms, stream);
+      case 32:  return launch_width<32>(a, splits, dev.sms, stream);
+      case 64:  return launch_width<64>(a, splits, dev.sms, stream);
+      case 128: return launch_width<128>(a, splits, dev.sms, stream);
+      default:  return launch_width<256>(a, splits, dev.sms, stream);
+   }
+}
+
+static Side side_of(const solid_gpu_blocks *b, size_t rows)
+{
+   return { (const uint8_t *)b->codes, (int64_t)b->ld, b->scales, (int64_t)b->scale_stride0 / 4, (int64_t)b->scale_stride1 / 4,
+            (int64_t)rows, b->block == 1 ? 0 : 7, b->format };
+}
+
+} // namespace sd
+
+extern "C" int solid_gpu_block_gemm(int ctype, size_t M, size_t N, size_t K, const solid_gpu_blocks *a, const solid_gpu_blocks *b,
+                                    const solid_gpu_matrix *c, cudaStream_t stream)
+{
+   const char *op = "block_gemm";
+   if (ctype != SD_HALF && ctype != SD_FLOAT) SD_ERROR("%s: the result's type must be half or float", op);
+   if (M > ((size_t)1 << 40) || N > ((size_t)1 << 40) || K > ((size_t)1 << 40)) SD_ERROR("%s: matrix too large", op);
+   if (sd::check_blocks(a, op, "a") != 0 || sd::check_blocks(b, op, "b") != 0) return -1;
+   if (c == nullptr || c->ptr == nullptr) SD_ERROR("%s: missing matrix c", op);
+   const ptrdiff_t es = solid_gpu_type_size[ctype];
+   if ((uintptr_t)c->ptr % es != 0 || c->stride0 % es != 0 || c->stride1 % es != 0) SD_ERROR("%s: matrix c must be aligned to its element size", op);
+   if (M == 0 || N == 0) return 0;
+   sd::GemmArgs g = { sd::side_of(a, M), sd::side_of(b, N), (int64_t)K, (char *)c->ptr, (int64_t)c->stride0, (int64_t)c->stride1, ctype == SD_HALF };
+   return sd::gemm(g, stream);
+}

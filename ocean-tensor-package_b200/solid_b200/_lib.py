@@ -52,6 +52,20 @@ class Operand(C.Structure):
                 ("byteswapped", C.c_int)]
 
 
+class Matrix(C.Structure):
+    """solid_gpu_matrix of the row operators."""
+    _fields_ = [("ptr", C.c_void_p), ("stride0", C.c_ssize_t), ("stride1", C.c_ssize_t)]
+
+
+class BlocksView(C.Structure):
+    """solid_gpu_blocks: 8-bit codes with their scales."""
+    _fields_ = [("codes", C.c_void_p), ("ld", C.c_ssize_t), ("scales", C.c_void_p), ("scale_stride0", C.c_ssize_t),
+                ("scale_stride1", C.c_ssize_t), ("block", C.c_int), ("format", C.c_int)]
+
+
+FORMATS = {"e4m3": 0, "e5m2": 1}                       # SOLID_GPU_E4M3, SOLID_GPU_E5M2
+
+
 def _sizes(seq):
     return (C.c_size_t * max(len(seq), 1))(*seq)
 
@@ -305,6 +319,47 @@ class SolidGPU:
         f = self.fn("solid_gpu_mixed_multiply_add")
         self._check(f(C.c_int(len(size)), _sizes(size), C.byref(ops[0]), C.byref(ops[1]), C.byref(ops[2]),
                       C.byref(ops[3]), C.c_int(dt.INDEX[ctype]), C.c_void_p(stream)), "mixed_multiply_add")
+
+    # -- the 8-bit linear layer ----------------------------------------------------------
+    # Matrices are Matrix or BlocksView structures, None where they are absent.
+    def _typed(self, name, *argtypes):
+        f = getattr(self.dll, name)
+        if f.argtypes is None:
+            f.argtypes, f.restype = argtypes, C.c_int
+        return f
+
+    def rms_norm(self, dtype, n, rows, x, residual, weight, eps, h, y, stream=0):
+        m = C.POINTER(Matrix)
+        f = self._typed("solid_gpu_rms_norm", C.c_int, C.c_size_t, C.c_size_t, m, m, C.c_void_p, C.c_double, m, m, C.c_void_p)
+        self._check(f(dt.INDEX[dtype], n, rows, x, residual, weight, eps, h, y, stream), "rms_norm")
+
+    def rms_norm_quantize(self, dtype, n, rows, x, residual, weight, eps, h, y, stream=0):
+        m = C.POINTER(Matrix)
+        f = self._typed("solid_gpu_rms_norm_quantize", C.c_int, C.c_size_t, C.c_size_t, m, m, C.c_void_p, C.c_double, m,
+                        C.POINTER(BlocksView), C.c_void_p)
+        self._check(f(dt.INDEX[dtype], n, rows, x, residual, weight, eps, h, y, stream), "rms_norm_quantize")
+
+    def rms_norm_grad_buffer_size(self, dtype, n, rows, device: int) -> int:
+        out = C.c_size_t(0)
+        f = self._typed("solid_gpu_rms_norm_grad_buffer_size", C.c_int, C.c_size_t, C.c_size_t, C.c_int, C.POINTER(C.c_size_t))
+        self._check(f(dt.INDEX[dtype], n, rows, device, C.byref(out)), "rms_norm_grad_buffer_size")
+        return out.value
+
+    def rms_norm_grad(self, dtype, n, rows, dy, h, weight, eps, dres, dh, dweight, buffer, stream=0):
+        m = C.POINTER(Matrix)
+        f = self._typed("solid_gpu_rms_norm_grad", C.c_int, C.c_size_t, C.c_size_t, m, m, C.c_void_p, C.c_double, m, m,
+                        C.c_void_p, C.c_void_p, C.c_void_p)
+        self._check(f(dt.INDEX[dtype], n, rows, dy, h, weight, eps, dres, dh, dweight, buffer, stream), "rms_norm_grad")
+
+    def block_quantize(self, dtype, n, rows, x, y, stream=0):
+        f = self._typed("solid_gpu_block_quantize", C.c_int, C.c_size_t, C.c_size_t, C.POINTER(Matrix), C.POINTER(BlocksView),
+                        C.c_void_p)
+        self._check(f(dt.INDEX[dtype], n, rows, x, y, stream), "block_quantize")
+
+    def block_gemm(self, ctype, m, n, k, a, b, c, stream=0):
+        v = C.POINTER(BlocksView)
+        f = self._typed("solid_gpu_block_gemm", C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, v, v, C.POINTER(Matrix), C.c_void_p)
+        self._check(f(dt.INDEX[ctype], m, n, k, a, b, c, stream), "block_gemm")
 
 
 _instance: SolidGPU | None = None

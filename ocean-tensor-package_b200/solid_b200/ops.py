@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import builtins as _py
 import struct
+from typing import NamedTuple
 
 import numpy as np
 
@@ -465,3 +466,234 @@ def fill_at(t: Tensor, positions, value) -> Tensor:
     sv = _ocean.get().scalar(scalar_bytes(value, t.dtype), t.dtype)
     _dispatch("fillIndex", C.byref(ix), C.byref(sv))
     return t
+
+
+# ----------------------------------------------------------------------------
+# the 8-bit linear layer: norm, conversion to 8 bits with scales, product
+# ----------------------------------------------------------------------------
+# A matrix [n, rows] is column-major like every tensor: a row (a token) is n elements side by side, and dimension 0 is
+# the one that a norm or a block of 128 runs along.  Further dimensions count as rows.  Half, float and double; results
+# are rounded once, to nearest even, with subnormals (the copy family rounds as the reference's CPU code does).
+class Blocks(NamedTuple):
+    """8-bit floating-point codes with scales: element (i, row) stands for codes[i, row] * scales[row // block, i // 128].
+
+    codes    uint8 tensor [n, rows], stride 1 along dimension 0 (rows on 16-byte boundaries reach the tensor cores)
+    scales   float tensor [rows, ceil(n / 128)], or [ceil(rows / 128), ceil(n / 128)] where 128 rows share a scale
+    format   "e4m3" or "e5m2"
+    """
+    codes: Tensor
+    scales: Tensor
+    format: str = "e4m3"
+
+
+def _format(name: str) -> int:
+    if name not in _lib.FORMATS:
+        raise ValueError("unknown 8-bit format %r: e4m3 or e5m2" % (name,))
+    return _lib.FORMATS[name]
+
+
+def _as_rows(t: Tensor):
+    """(rows, stride of a row) of a tensor whose dimensions 1.. step evenly, None where they do not."""
+    rows, step = 1, 0
+    for s, st in zip(t.size[1:], t.strides[1:]):
+        if s == 1:
+            continue
+        if rows == 1:
+            step = st
+        elif st != step * rows:
+            return None
+        rows *= s
+    return (0 if 0 in t.size[1:] else rows), step
+
+
+def _matrix(t: Tensor):
+    """The tensor and its Matrix; one whose trailing dimensions do not step evenly is copied first."""
+    r = _as_rows(t)
+    if r is None:
+        t = clone(t)
+        r = _as_rows(t)
+    return t, _lib.Matrix(t.ptr, t.strides[0], r[1])
+
+
+def _row_operand(t: Tensor, like: Tensor, what: str) -> Tensor:
+    if t.storage.device != like.storage.device:
+        raise ValueError("%s is on another device" % what)
+    return _prepared(t, like.dtype, like.size)
+
+
+def _row_input(x: Tensor, what: str) -> Tensor:
+    if x.dtype not in ("half", "float", "double"):
+        raise TypeError("%s is not available for type %s" % (what, x.dtype))
+    if x.ndims < 1:
+        raise ValueError("%s needs at least one dimension" % what)
+    return _native(x)
+
+
+def _norm_weight(weight, x: Tensor):
+    if weight is None:
+        return None
+    if weight.size != x.size[:1]:
+        raise ValueError("the weights need size [%d]" % x.size[0])
+    if weight.storage.device != x.storage.device:
+        raise ValueError("weight is on another device")
+    w = _prepared(weight, x.dtype, weight.size)
+    return w if w.size[0] <= 1 or w.strides[0] == w.elemsize else clone(w)
+
+
+def _result(dst, like: Tensor, dtype: str):
+    """Where a kernel writes: dst itself where it is native and steps evenly, else a new tensor that is copied there."""
+    if dst is not None:
+        if dst.size != like.size:
+            raise ValueError("the result has size %s, not %s" % (like.size, dst.size))
+        if dst.storage.device != like.storage.device:
+            raise ValueError("the result is on another device")
+        if dst.dtype == dtype and not dst.byteswapped and _as_rows(dst) is not None and \
+                dst.ptr % dst.elemsize == 0 and _py.all(s % dst.elemsize == 0 for s in dst.strides) and \
+                _py.all(st != 0 or s <= 1 for s, st in zip(dst.size, dst.strides)):
+            return dst
+    return Tensor.empty(like.size, dtype, like.storage.device)
+
+
+def _delivered(out: Tensor, dst) -> Tensor:
+    return out if dst is None or out is dst else copy(out, dst)
+
+
+def _norm_call(x, weight, eps, residual, h, what):
+    """What rms_norm and rms_norm_quantize share: operands, their matrices, and the tensor for h."""
+    import ctypes as C
+    x, mx = _matrix(_row_input(x, what))
+    w = _norm_weight(weight, x)
+    mr = mh = res = total = None
+    if residual is not None:
+        res, mr = _matrix(_row_operand(residual, x, "residual"))
+        mr = C.byref(mr)
+        total = _result(h, x, x.dtype)
+    elif h is not None:
+        raise ValueError("h is x + residual: there is no residual")
+    if total is not None:
+        mh = C.byref(_matrix(total)[1])
+    rows = _as_rows(x)[0]
+    return x, rows, C.byref(mx), mr, (w.ptr if w is not None else None), float(eps), mh, total, (w, res)
+
+
+def rms_norm(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residual: Tensor | None = None,
+             dst: Tensor | None = None, h: Tensor | None = None):
+    """Root-mean-square norm along dimension 0: y = x * weight / sqrt(mean(x^2) + eps).
+
+    With a residual the sum h = x + residual is normalised (before it is rounded) and returned too: (y, h).  dst and h
+    say where y and h go; h may be the residual's own tensor, dst that of x."""
+    import ctypes as C
+    x, rows, mx, mr, w, eps, mh, total, keep = _norm_call(x, weight, eps, residual, h, "rms_norm")
+    out = _result(dst, x, x.dtype)
+    _lib_for(x).rms_norm(x.dtype, x.size[0], rows, mx, mr, w, eps, mh, C.byref(_matrix(out)[1]), _stream(x))
+    y = _delivered(out, dst)
+    return y if total is None else (y, _delivered(total, h))
+
+
+def _empty_blocks(n: int, rows: int, block: int, format: str, device) -> Blocks:
+    """Room for codes (rows padded to 16 bytes) and scales."""
+    ld = (n + 15) // 16 * 16
+    codes = Tensor.empty([ld, rows], "uint8", device)
+    return Blocks(Tensor(codes.storage, "uint8", [n, rows], [1, ld]),
+                  Tensor.empty([(rows + block - 1) // block, (n + 127) // 128], "float", device), format)
+
+
+def _blocks_view(b: Blocks, what: str):
+    """(codes, BlocksView) of a caller's codes and scales, checked against each other."""
+    codes, scales = b.codes, b.scales
+    if codes.dtype != "uint8" or scales.dtype != "float" or scales.byteswapped:
+        raise TypeError("%s: codes are uint8, scales native floats" % what)
+    if codes.ndims != 2 or scales.ndims != 2:
+        raise ValueError("%s: codes and scales are matrices" % what)
+    if scales.storage.device != codes.storage.device:
+        raise ValueError("%s: codes and scales are on different devices" % what)
+    n, rows = codes.size
+    nb = (n + 127) // 128
+    if scales.size == [rows, nb]:
+        block = 1
+    elif scales.size == [(rows + 127) // 128, nb]:
+        block = 128
+    else:
+        raise ValueError("%s: scales of size %s do not belong to codes of size %s" % (what, scales.size, codes.size))
+    fmt = _format(b.format)
+    if n > 1 and codes.strides[0] != 1:
+        codes = clone(codes)
+    return codes, _lib.BlocksView(codes.ptr, codes.strides[1], scales.ptr, scales.strides[0], scales.strides[1], block, fmt)
+
+
+def rms_norm_quantize(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residual: Tensor | None = None,
+                      format: str = "e4m3", h: Tensor | None = None):
+    """rms_norm whose y is returned as Blocks, a scale for 128 elements of each row; with a residual (Blocks, h)."""
+    import ctypes as C
+    _format(format)
+    x, rows, mx, mr, w, eps, mh, total, keep = _norm_call(x, weight, eps, residual, h, "rms_norm_quantize")
+    out = _empty_blocks(x.size[0], rows, 1, format, x.storage.device)
+    _lib_for(x).rms_norm_quantize(x.dtype, x.size[0], rows, mx, mr, w, eps, mh, C.byref(_blocks_view(out, "y")[1]), _stream(x))
+    return out if total is None else (out, _delivered(total, h))
+
+
+def rms_norm_grad(dy: Tensor, h: Tensor, weight: Tensor | None = None, eps: float = 1e-6, dres: Tensor | None = None,
+                  dst: Tensor | None = None):
+    """Gradient of rms_norm at h (the input, or x + residual): returns (dh, dweight).
+
+    dres, the gradient that reaches h past the norm, is added to dh.  dweight is in the work type (half: float)."""
+    import ctypes as C
+    import torch
+    h, mh = _matrix(_row_input(h, "rms_norm_grad"))
+    if dy.size != h.size or (dres is not None and dres.size != h.size):
+        raise ValueError("gradients have the size of h, %s" % h.size)
+    g, mg = _matrix(_row_operand(dy, h, "dy"))
+    w = _norm_weight(weight, h)
+    mr = None
+    if dres is not None:
+        dres, mr = _matrix(_row_operand(dres, h, "dres"))
+        mr = C.byref(mr)
+    n, rows = h.size[0], _as_rows(h)[0]
+    out = _result(dst, h, h.dtype)
+    dweight = Tensor.empty([n], "double" if h.dtype == "double" else "float", h.storage.device)
+    lib = _lib_for(h)
+    # a buffer of its own for each call: calls on several streams and captured graphs share nothing
+    buf = torch.empty(max(lib.rms_norm_grad_buffer_size(h.dtype, n, rows, h.device_index), 16), dtype=torch.uint8,
+                      device=h.storage.device)
+    lib.rms_norm_grad(h.dtype, n, rows, C.byref(mg), C.byref(mh), w.ptr if w is not None else None, float(eps), mr,
+                      C.byref(_matrix(out)[1]), dweight.ptr, buf.data_ptr(), _stream(h))
+    return _delivered(out, dst), dweight
+
+
+def block_quantize(x: Tensor, block: int = 1, format: str = "e4m3") -> Blocks:
+    """8-bit codes of a matrix [n, rows] with a scale for 128 elements of dimension 0 by `block` (1 or 128) rows.
+
+    scale = max(largest magnitude / largest code, 2^-126); code = x / scale to nearest even.  Strides are free:
+    block_quantize(x.T) gives the codes of the transposed matrix."""
+    import ctypes as C
+    _format(format)
+    if block not in (1, 128):
+        raise ValueError("a scale belongs to 1 or 128 rows")
+    x, mx = _matrix(_row_input(x, "block_quantize"))
+    rows = _as_rows(x)[0]
+    out = _empty_blocks(x.size[0], rows, block, format, x.storage.device)
+    view = _blocks_view(out, "y")[1]
+    view.block = block
+    _lib_for(x).block_quantize(x.dtype, x.size[0], rows, C.byref(mx), C.byref(view), _stream(x))
+    return out
+
+
+def block_gemm(a: Blocks, b: Blocks, dtype: str = "half", dst: Tensor | None = None) -> Tensor:
+    """Product of 8-bit matrices with scales: c[m, n] = sum over k of a[k, m] b[k, n], half or float.
+
+    A linear layer with weights W [K, M] and tokens X [K, N] (both Blocks): y = block_gemm(W, X).  Its gradients:
+    dX = block_gemm(block_quantize(w.T, 128), block_quantize(dy)), and dW = block_gemm(block_quantize(x.T),
+    block_quantize(dy.T), "float"), a matrix [K, M]."""
+    import ctypes as C
+    if dtype not in ("half", "float"):
+        raise TypeError("block_gemm gives half or float, not %s" % dtype)
+    ka, va = _blocks_view(a, "a")
+    kb, vb = _blocks_view(b, "b")
+    if ka.size[0] != kb.size[0]:
+        raise ValueError("block_gemm: depths %d and %d differ" % (ka.size[0], kb.size[0]))
+    if ka.storage.device != kb.storage.device:
+        raise ValueError("block_gemm: operands on different devices")
+    m, n, k = ka.size[1], kb.size[1], ka.size[0]
+    out = _result(dst, Tensor(ka.storage, dtype, [m, n]), dtype)
+    _lib_for(ka).block_gemm(dtype, m, n, k, C.byref(va), C.byref(vb), C.byref(_matrix(out)[1]), _stream(ka))
+    return _delivered(out, dst)
