@@ -7,6 +7,7 @@ Python sequences; strides are in bytes.
 from __future__ import annotations
 
 import ctypes as C
+from functools import cached_property
 from pathlib import Path
 
 from . import dtypes as dt
@@ -322,44 +323,45 @@ class SolidGPU:
 
     # -- the 8-bit linear layer ----------------------------------------------------------
     # Matrices are Matrix or BlocksView structures, None where they are absent.
+    # A call takes the typed function once from the library and passes plain Python numbers and structures.
     def _typed(self, name, *argtypes):
         f = getattr(self.dll, name)
-        if f.argtypes is None:
-            f.argtypes, f.restype = argtypes, C.c_int
+        f.argtypes, f.restype = argtypes, C.c_int
         return f
 
+    @cached_property
+    def _layer(self):
+        """The layer's functions with their argument types."""
+        i, z, d, p, m, v = C.c_int, C.c_size_t, C.c_double, C.c_void_p, C.POINTER(Matrix), C.POINTER(BlocksView)
+        return {"rms_norm": self._typed("solid_gpu_rms_norm", i, z, z, m, m, p, d, m, m, p),
+                "rms_norm_quantize": self._typed("solid_gpu_rms_norm_quantize", i, z, z, m, m, p, d, m, v, p),
+                "rms_norm_grad_buffer_size": self._typed("solid_gpu_rms_norm_grad_buffer_size", i, z, z, i, C.POINTER(z)),
+                "rms_norm_grad": self._typed("solid_gpu_rms_norm_grad", i, z, z, m, m, p, d, m, m, p, p, p),
+                "block_quantize": self._typed("solid_gpu_block_quantize", i, z, z, m, v, p),
+                "block_gemm": self._typed("solid_gpu_block_gemm", i, z, z, z, v, v, m, p)}
+
     def rms_norm(self, dtype, n, rows, x, residual, weight, eps, h, y, stream=0):
-        m = C.POINTER(Matrix)
-        f = self._typed("solid_gpu_rms_norm", C.c_int, C.c_size_t, C.c_size_t, m, m, C.c_void_p, C.c_double, m, m, C.c_void_p)
-        self._check(f(dt.INDEX[dtype], n, rows, x, residual, weight, eps, h, y, stream), "rms_norm")
+        self._check(self._layer["rms_norm"](dt.INDEX[dtype], n, rows, x, residual, weight, eps, h, y, stream), "rms_norm")
 
     def rms_norm_quantize(self, dtype, n, rows, x, residual, weight, eps, h, y, stream=0):
-        m = C.POINTER(Matrix)
-        f = self._typed("solid_gpu_rms_norm_quantize", C.c_int, C.c_size_t, C.c_size_t, m, m, C.c_void_p, C.c_double, m,
-                        C.POINTER(BlocksView), C.c_void_p)
-        self._check(f(dt.INDEX[dtype], n, rows, x, residual, weight, eps, h, y, stream), "rms_norm_quantize")
+        self._check(self._layer["rms_norm_quantize"](dt.INDEX[dtype], n, rows, x, residual, weight, eps, h, y, stream),
+                    "rms_norm_quantize")
 
     def rms_norm_grad_buffer_size(self, dtype, n, rows, device: int) -> int:
         out = C.c_size_t(0)
-        f = self._typed("solid_gpu_rms_norm_grad_buffer_size", C.c_int, C.c_size_t, C.c_size_t, C.c_int, C.POINTER(C.c_size_t))
-        self._check(f(dt.INDEX[dtype], n, rows, device, C.byref(out)), "rms_norm_grad_buffer_size")
+        self._check(self._layer["rms_norm_grad_buffer_size"](dt.INDEX[dtype], n, rows, device, C.byref(out)),
+                    "rms_norm_grad_buffer_size")
         return out.value
 
     def rms_norm_grad(self, dtype, n, rows, dy, h, weight, eps, dres, dh, dweight, buffer, stream=0):
-        m = C.POINTER(Matrix)
-        f = self._typed("solid_gpu_rms_norm_grad", C.c_int, C.c_size_t, C.c_size_t, m, m, C.c_void_p, C.c_double, m, m,
-                        C.c_void_p, C.c_void_p, C.c_void_p)
-        self._check(f(dt.INDEX[dtype], n, rows, dy, h, weight, eps, dres, dh, dweight, buffer, stream), "rms_norm_grad")
+        self._check(self._layer["rms_norm_grad"](dt.INDEX[dtype], n, rows, dy, h, weight, eps, dres, dh, dweight, buffer, stream),
+                    "rms_norm_grad")
 
     def block_quantize(self, dtype, n, rows, x, y, stream=0):
-        f = self._typed("solid_gpu_block_quantize", C.c_int, C.c_size_t, C.c_size_t, C.POINTER(Matrix), C.POINTER(BlocksView),
-                        C.c_void_p)
-        self._check(f(dt.INDEX[dtype], n, rows, x, y, stream), "block_quantize")
+        self._check(self._layer["block_quantize"](dt.INDEX[dtype], n, rows, x, y, stream), "block_quantize")
 
     def block_gemm(self, ctype, m, n, k, a, b, c, stream=0):
-        v = C.POINTER(BlocksView)
-        f = self._typed("solid_gpu_block_gemm", C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, v, v, C.POINTER(Matrix), C.c_void_p)
-        self._check(f(dt.INDEX[ctype], m, n, k, a, b, c, stream), "block_gemm")
+        self._check(self._layer["block_gemm"](dt.INDEX[ctype], m, n, k, a, b, c, stream), "block_gemm")
 
 
 _instance: SolidGPU | None = None

@@ -506,74 +506,75 @@ def _as_rows(t: Tensor):
     return (0 if 0 in t.size[1:] else rows), step
 
 
-def _matrix(t: Tensor):
-    """The tensor and its Matrix; one whose trailing dimensions do not step evenly is copied first."""
+# A single token's call is a few microseconds of work on the GPU, so the host's part is kept as short: matrices that
+# the kernels take as they are pass one test, everything else goes the general way through _prepared and clone.
+def _row_operand(t: Tensor, dtype: str, size, device, what: str):
+    """An operand as the kernels take it, the number of its rows, and its Matrix: of the given type, native, aligned, its
+    rows a step apart."""
+    if t.storage.device != device:
+        raise ValueError("%s is on another device" % what)
+    if t.dtype == dtype and len(size) == 2 and t.size == size and not t.byteswapped:
+        s0, s1 = t.strides
+        p = t.storage.data_ptr() + t.offset
+        if not (p | s0 | s1) & (dt.SIZE[dtype] - 1):
+            return t, size[1], _lib.Matrix(p, s0, s1)
+    t = _prepared(t, dtype, size)
     r = _as_rows(t)
     if r is None:
         t = clone(t)
         r = _as_rows(t)
-    return t, _lib.Matrix(t.ptr, t.strides[0], r[1])
+    return t, r[0], _lib.Matrix(t.ptr, t.strides[0], r[1])
 
 
-def _row_operand(t: Tensor, like: Tensor, what: str) -> Tensor:
-    if t.storage.device != like.storage.device:
-        raise ValueError("%s is on another device" % what)
-    return _prepared(t, like.dtype, like.size)
-
-
-def _row_input(x: Tensor, what: str) -> Tensor:
+def _row_input(x: Tensor, what: str):
     if x.dtype not in ("half", "float", "double"):
         raise TypeError("%s is not available for type %s" % (what, x.dtype))
-    if x.ndims < 1:
+    if not x.size:
         raise ValueError("%s needs at least one dimension" % what)
-    return _native(x)
+    return _row_operand(x, x.dtype, x.size, x.storage.device, "the input")
 
 
 def _norm_weight(weight, x: Tensor):
+    """The weights as the kernels take them (contiguous, in the type of x) and their address."""
     if weight is None:
-        return None
+        return None, None
     if weight.size != x.size[:1]:
         raise ValueError("the weights need size [%d]" % x.size[0])
     if weight.storage.device != x.storage.device:
         raise ValueError("weight is on another device")
     w = _prepared(weight, x.dtype, weight.size)
-    return w if w.size[0] <= 1 or w.strides[0] == w.elemsize else clone(w)
+    if w.size[0] > 1 and w.strides[0] != w.elemsize:
+        w = clone(w)
+    return w, w.storage.data_ptr() + w.offset
 
 
-def _result(dst, like: Tensor, dtype: str):
-    """Where a kernel writes: dst itself where it is native and steps evenly, else a new tensor that is copied there."""
+def _result(dst, size, dtype: str, device):
+    """Where a kernel writes, and its Matrix: dst itself where the kernel can, else a new tensor that is copied there."""
     if dst is not None:
-        if dst.size != like.size:
-            raise ValueError("the result has size %s, not %s" % (like.size, dst.size))
-        if dst.storage.device != like.storage.device:
+        if dst.size != size:
+            raise ValueError("the result has size %s, not %s" % (size, dst.size))
+        if dst.storage.device != device:
             raise ValueError("the result is on another device")
-        if dst.dtype == dtype and not dst.byteswapped and _as_rows(dst) is not None and \
+        r = _as_rows(dst)
+        if dst.dtype == dtype and not dst.byteswapped and r is not None and \
                 dst.ptr % dst.elemsize == 0 and _py.all(s % dst.elemsize == 0 for s in dst.strides) and \
                 _py.all(st != 0 or s <= 1 for s, st in zip(dst.size, dst.strides)):
-            return dst
-    return Tensor.empty(like.size, dtype, like.storage.device)
+            return dst, _lib.Matrix(dst.ptr, dst.strides[0], r[1])
+    out = Tensor.empty(size, dtype, device)
+    es = dt.SIZE[dtype]
+    return out, _lib.Matrix(out.storage.data_ptr(), es, es * size[0])
 
 
 def _delivered(out: Tensor, dst) -> Tensor:
     return out if dst is None or out is dst else copy(out, dst)
 
 
-def _norm_call(x, weight, eps, residual, h, what):
-    """What rms_norm and rms_norm_quantize share: operands, their matrices, and the tensor for h."""
-    import ctypes as C
-    x, mx = _matrix(_row_input(x, what))
-    w = _norm_weight(weight, x)
-    mr = mh = res = total = None
-    if residual is not None:
-        res, mr = _matrix(_row_operand(residual, x, "residual"))
-        mr = C.byref(mr)
-        total = _result(h, x, x.dtype)
-    elif h is not None:
-        raise ValueError("h is x + residual: there is no residual")
-    if total is not None:
-        mh = C.byref(_matrix(total)[1])
-    rows = _as_rows(x)[0]
-    return x, rows, C.byref(mx), mr, (w.ptr if w is not None else None), float(eps), mh, total, (w, res)
+def _here(device):
+    """The library with the tensors' device current, and that device's current stream."""
+    import torch
+    if torch.cuda.current_device() != device.index:
+        torch.cuda.set_device(device)
+    return _lib.get(), torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def rms_norm(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residual: Tensor | None = None,
@@ -582,20 +583,38 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residua
 
     With a residual the sum h = x + residual is normalised (before it is rounded) and returned too: (y, h).  dst and h
     say where y and h go; h may be the residual's own tensor, dst that of x."""
-    import ctypes as C
-    x, rows, mx, mr, w, eps, mh, total, keep = _norm_call(x, weight, eps, residual, h, "rms_norm")
-    out = _result(dst, x, x.dtype)
-    _lib_for(x).rms_norm(x.dtype, x.size[0], rows, mx, mr, w, eps, mh, C.byref(_matrix(out)[1]), _stream(x))
+    x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, "rms_norm")
+    device = x.storage.device
+    out, my = _result(dst, x.size, x.dtype, device)
+    lib, stream = _here(device)
+    lib.rms_norm(x.dtype, x.size[0], rows, mx, mr, pw, eps, mh, my, stream)
     y = _delivered(out, dst)
     return y if total is None else (y, _delivered(total, h))
 
 
-def _empty_blocks(n: int, rows: int, block: int, format: str, device) -> Blocks:
-    """Room for codes (rows padded to 16 bytes) and scales."""
+def _norm_operands(x, weight, residual, h, what):
+    """What rms_norm and rms_norm_quantize share.  The tensors are returned beside their addresses to keep them alive."""
+    x, rows, mx = _row_input(x, what)
+    w, pw = _norm_weight(weight, x)
+    if residual is None:
+        if h is not None:
+            raise ValueError("h is x + residual: there is no residual")
+        return x, rows, mx, None, None, w, pw, None, None
+    device = x.storage.device
+    res, _, mr = _row_operand(residual, x.dtype, x.size, device, "residual")
+    total, mh = _result(h, x.size, x.dtype, device)
+    return x, rows, mx, res, mr, w, pw, total, mh
+
+
+def _empty_blocks(n: int, rows: int, block: int, format: str, device):
+    """Room for codes (rows padded to 16 bytes) and scales, and its BlocksView."""
     ld = (n + 15) // 16 * 16
+    rb = (rows + block - 1) // block
     codes = Tensor.empty([ld, rows], "uint8", device)
-    return Blocks(Tensor(codes.storage, "uint8", [n, rows], [1, ld]),
-                  Tensor.empty([(rows + block - 1) // block, (n + 127) // 128], "float", device), format)
+    codes.size[0] = n
+    scales = Tensor.empty([rb, (n + 127) // 128], "float", device)
+    return Blocks(codes, scales, format), _lib.BlocksView(codes.storage.data_ptr(), ld, scales.storage.data_ptr(), 4, 4 * rb,
+                                                          block, _lib.FORMATS[format])
 
 
 def _blocks_view(b: Blocks, what: str):
@@ -603,7 +622,7 @@ def _blocks_view(b: Blocks, what: str):
     codes, scales = b.codes, b.scales
     if codes.dtype != "uint8" or scales.dtype != "float" or scales.byteswapped:
         raise TypeError("%s: codes are uint8, scales native floats" % what)
-    if codes.ndims != 2 or scales.ndims != 2:
+    if len(codes.size) != 2 or len(scales.size) != 2:
         raise ValueError("%s: codes and scales are matrices" % what)
     if scales.storage.device != codes.storage.device:
         raise ValueError("%s: codes and scales are on different devices" % what)
@@ -618,17 +637,19 @@ def _blocks_view(b: Blocks, what: str):
     fmt = _format(b.format)
     if n > 1 and codes.strides[0] != 1:
         codes = clone(codes)
-    return codes, _lib.BlocksView(codes.ptr, codes.strides[1], scales.ptr, scales.strides[0], scales.strides[1], block, fmt)
+    return codes, _lib.BlocksView(codes.storage.data_ptr() + codes.offset, codes.strides[1],
+                                  scales.storage.data_ptr() + scales.offset, scales.strides[0], scales.strides[1], block, fmt)
 
 
 def rms_norm_quantize(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residual: Tensor | None = None,
                       format: str = "e4m3", h: Tensor | None = None):
     """rms_norm whose y is returned as Blocks, a scale for 128 elements of each row; with a residual (Blocks, h)."""
-    import ctypes as C
     _format(format)
-    x, rows, mx, mr, w, eps, mh, total, keep = _norm_call(x, weight, eps, residual, h, "rms_norm_quantize")
-    out = _empty_blocks(x.size[0], rows, 1, format, x.storage.device)
-    _lib_for(x).rms_norm_quantize(x.dtype, x.size[0], rows, mx, mr, w, eps, mh, C.byref(_blocks_view(out, "y")[1]), _stream(x))
+    x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, "rms_norm_quantize")
+    device = x.storage.device
+    out, view = _empty_blocks(x.size[0], rows, 1, format, device)
+    lib, stream = _here(device)
+    lib.rms_norm_quantize(x.dtype, x.size[0], rows, mx, mr, pw, eps, mh, view, stream)
     return out if total is None else (out, _delivered(total, h))
 
 
@@ -637,26 +658,22 @@ def rms_norm_grad(dy: Tensor, h: Tensor, weight: Tensor | None = None, eps: floa
     """Gradient of rms_norm at h (the input, or x + residual): returns (dh, dweight).
 
     dres, the gradient that reaches h past the norm, is added to dh.  dweight is in the work type (half: float)."""
-    import ctypes as C
     import torch
-    h, mh = _matrix(_row_input(h, "rms_norm_grad"))
+    h, rows, mh = _row_input(h, "rms_norm_grad")
     if dy.size != h.size or (dres is not None and dres.size != h.size):
         raise ValueError("gradients have the size of h, %s" % h.size)
-    g, mg = _matrix(_row_operand(dy, h, "dy"))
-    w = _norm_weight(weight, h)
+    device, dtype, n = h.storage.device, h.dtype, h.size[0]
+    dy, _, mg = _row_operand(dy, dtype, h.size, device, "dy")
+    w, pw = _norm_weight(weight, h)
     mr = None
     if dres is not None:
-        dres, mr = _matrix(_row_operand(dres, h, "dres"))
-        mr = C.byref(mr)
-    n, rows = h.size[0], _as_rows(h)[0]
-    out = _result(dst, h, h.dtype)
-    dweight = Tensor.empty([n], "double" if h.dtype == "double" else "float", h.storage.device)
-    lib = _lib_for(h)
+        dres, _, mr = _row_operand(dres, dtype, h.size, device, "dres")
+    out, mo = _result(dst, h.size, dtype, device)
+    dweight = Tensor.empty([n], "double" if dtype == "double" else "float", device)
+    lib, stream = _here(device)
     # a buffer of its own for each call: calls on several streams and captured graphs share nothing
-    buf = torch.empty(max(lib.rms_norm_grad_buffer_size(h.dtype, n, rows, h.device_index), 16), dtype=torch.uint8,
-                      device=h.storage.device)
-    lib.rms_norm_grad(h.dtype, n, rows, C.byref(mg), C.byref(mh), w.ptr if w is not None else None, float(eps), mr,
-                      C.byref(_matrix(out)[1]), dweight.ptr, buf.data_ptr(), _stream(h))
+    buf = torch.empty(lib.rms_norm_grad_buffer_size(dtype, n, rows, device.index) + 16, dtype=torch.uint8, device=device)
+    lib.rms_norm_grad(dtype, n, rows, mg, mh, pw, eps, mr, mo, dweight.storage.data_ptr(), buf.data_ptr(), stream)
     return _delivered(out, dst), dweight
 
 
@@ -665,16 +682,14 @@ def block_quantize(x: Tensor, block: int = 1, format: str = "e4m3") -> Blocks:
 
     scale = max(largest magnitude / largest code, 2^-126); code = x / scale to nearest even.  Strides are free:
     block_quantize(x.T) gives the codes of the transposed matrix."""
-    import ctypes as C
     _format(format)
     if block not in (1, 128):
         raise ValueError("a scale belongs to 1 or 128 rows")
-    x, mx = _matrix(_row_input(x, "block_quantize"))
-    rows = _as_rows(x)[0]
-    out = _empty_blocks(x.size[0], rows, block, format, x.storage.device)
-    view = _blocks_view(out, "y")[1]
-    view.block = block
-    _lib_for(x).block_quantize(x.dtype, x.size[0], rows, C.byref(mx), C.byref(view), _stream(x))
+    x, rows, mx = _row_input(x, "block_quantize")
+    device = x.storage.device
+    out, view = _empty_blocks(x.size[0], rows, block, format, device)
+    lib, stream = _here(device)
+    lib.block_quantize(x.dtype, x.size[0], rows, mx, view, stream)
     return out
 
 
@@ -684,16 +699,18 @@ def block_gemm(a: Blocks, b: Blocks, dtype: str = "half", dst: Tensor | None = N
     A linear layer with weights W [K, M] and tokens X [K, N] (both Blocks): y = block_gemm(W, X).  Its gradients:
     dX = block_gemm(block_quantize(w.T, 128), block_quantize(dy)), and dW = block_gemm(block_quantize(x.T),
     block_quantize(dy.T), "float"), a matrix [K, M]."""
-    import ctypes as C
     if dtype not in ("half", "float"):
         raise TypeError("block_gemm gives half or float, not %s" % dtype)
     ka, va = _blocks_view(a, "a")
     kb, vb = _blocks_view(b, "b")
-    if ka.size[0] != kb.size[0]:
-        raise ValueError("block_gemm: depths %d and %d differ" % (ka.size[0], kb.size[0]))
-    if ka.storage.device != kb.storage.device:
+    k, m = ka.size
+    device = ka.storage.device
+    if kb.size[0] != k:
+        raise ValueError("block_gemm: depths %d and %d differ" % (k, kb.size[0]))
+    if kb.storage.device != device:
         raise ValueError("block_gemm: operands on different devices")
-    m, n, k = ka.size[1], kb.size[1], ka.size[0]
-    out = _result(dst, Tensor(ka.storage, dtype, [m, n]), dtype)
-    _lib_for(ka).block_gemm(dtype, m, n, k, C.byref(va), C.byref(vb), C.byref(_matrix(out)[1]), _stream(ka))
+    n = kb.size[1]
+    out, mc = _result(dst, [m, n], dtype, device)
+    lib, stream = _here(device)
+    lib.block_gemm(dtype, m, n, k, va, vb, mc, stream)
     return _delivered(out, dst)
