@@ -25,10 +25,11 @@ template <> struct Held<double> { using type = float; };
 // ACROSS: the source is contiguous along the rows' dimension.  VEC: runs of eight start on 16-byte boundaries.
 // RB: rows that share a scale.
 template <class T, bool ACROSS, bool VEC, int RB>
-__global__ void __launch_bounds__(256, 2) quantize_tiles(const __grid_constant__ QuantArgs a)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tiles(const __grid_constant__ QuantArgs a)
 {
    using H = typename Held<T>::type;
    __shared__ uint32_t most[QT];
+   __shared__ alignas(16) float inverse[QT];
    __shared__ alignas(16) unsigned char turned[ACROSS ? QT * QT : 16];
    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, lane = threadIdx.x & 31;
    const int64_t ntiles = (a.n + QT - 1) / QT, rtiles = (a.rows + QT - 1) / QT;
@@ -90,9 +91,14 @@ __global__ void __launch_bounds__(256, 2) quantize_tiles(const __grid_constant__
          if (lane < 16) atomicMax(&most[along(j)], m);
       }
       __syncthreads();
+      if (threadIdx.x < QT) {
+         const float s = b8_scale(most[threadIdx.x], a.format);
+         inverse[threadIdx.x] = 1.0f / s;
+         if (threadIdx.x < along_left) store_scale(r0 + threadIdx.x, s);
+      }
+      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; j++) inv[j] = 1.0f / b8_scale(most[along(j)], a.format);
-      if (threadIdx.x < QT && threadIdx.x < along_left) store_scale(r0 + threadIdx.x, b8_scale(most[threadIdx.x], a.format));
+      for (int j = 0; j < 8; j++) inv[j] = inverse[along(j)];
    } else {                                               // a row is one p of 16 lanes
 #pragma unroll
       for (int p = 0; p < 8; p++) {

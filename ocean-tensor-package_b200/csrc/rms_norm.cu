@@ -13,6 +13,7 @@
 // reduction's barrier.
 #include <atomic>
 #include "block8.cuh"
+#include "tcgen05.cuh"
 
 namespace sd {
 
@@ -207,6 +208,107 @@ __global__ void __launch_bounds__(MAXT) norm_rows(const __grid_constant__ NormAr
    }
 }
 
+// ---------------------------------------------------------------------------
+// rows through a ring in shared memory
+// ---------------------------------------------------------------------------
+// Whole rows on 16-byte boundaries come by bulk copies into a ring of `stages` rows (of each operand), so that the loads in
+// flight do not depend on registers or on the reduction's barrier: one thread refills a row's place after the barrier
+// of the next row, by which time every thread has finished with it.  A wait that runs out makes the thread's sums NaN,
+// and with them the row.
+constexpr int RING_MAX = 4;
+
+struct Ring {
+   uint32_t bars, data, stage;                            // shared addresses, bytes of a stage
+   int stages;
+   bool ok;
+   __device__ __forceinline__ void start(char *smem, uint64_t *bar, int bytes, int count)
+   {
+      bars = tc::smem_u32(bar); data = tc::smem_u32(smem); stage = bytes; stages = count; ok = true;
+      if (threadIdx.x == 0) {
+         for (int s = 0; s < stages; s++) tc::bar_init(bars + 8 * s, 1);
+         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      }
+      __syncthreads();
+   }
+   // one row of an operand to its place in a stage
+   __device__ __forceinline__ void copy(int s, int offset, const RowMatrix &m, int64_t row, uint32_t bytes)
+   {
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   :: "r"(data + s * stage + offset), "l"(m.p + row * m.s1), "r"(bytes), "r"(bars + 8 * s) : "memory");
+   }
+   __device__ __forceinline__ void wait(int it) { if (ok) ok = tc::bar_wait(bars + 8 * (it % stages), (it / stages) & 1); }
+};
+
+template <class T, int V, bool QUANT, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_ring(const __grid_constant__ NormArgs a, int stages)
+{
+   using W = typename Real<T>::acc;
+   extern __shared__ __align__(128) char smem[];
+   __shared__ alignas(8) uint64_t bar[RING_MAX];
+   __shared__ W sums[2][32];
+   const int lane = threadIdx.x & 31, t = threadIdx.x, threads = blockDim.x;
+   const bool has_res = a.res.p != nullptr;
+   const int bytes = (int)(a.n * sizeof(T));
+   Ring ring;
+   ring.start(smem, bar, has_res ? 2 * bytes : bytes, stages);
+   auto load = [&](int it) {
+      const int64_t row = blockIdx.x + (int64_t)it * gridDim.x;
+      if (row >= a.rows) return;
+      const int s = it % stages;
+      tc::bar_expect(ring.bars + 8 * s, ring.stage);
+      ring.copy(s, 0, a.x, row, bytes);
+      if (has_res) ring.copy(s, bytes, a.res, row, bytes);
+   };
+   if (t == 0) for (int it = 0; it < stages; it++) load(it);
+   Eight<T> w[V];
+#pragma unroll
+   for (int v = 0; v < V; v++) fetch_weights<T, true>(w[v], a.w, chunk_first<true>(v, threads, t), a.n);
+   int it = 0;
+   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, it++) {
+      ring.wait(it);
+      const char *place = smem + (it % stages) * ring.stage;
+      W h[V][8];
+      W s = 0;
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+         const int i = (v * threads + t) * 8;
+         if (i < a.n) {
+            const Eight<T> x = load_eight<T>(place + i * sizeof(T));
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[v][j] = to_acc(x.e[j]);
+            if (has_res) {
+               const Eight<T> r = load_eight<T>(place + bytes + i * sizeof(T));
+#pragma unroll
+               for (int j = 0; j < 8; j++) h[v][j] += to_acc(r.e[j]);
+            }
+         } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[v][j] = 0;
+         }
+#pragma unroll
+         for (int j = 0; j < 8; j++) s = fma(h[v][j], h[v][j], s);
+      }
+      if (!ring.ok) s = (W)NAN;
+      s = row_sum<true>(s, threads, 0xFFFFFFFFu, sums[it & 1]);
+      if (t == 0 && it > 0) load(it - 1 + stages);
+      const W rr = (W)1 / sqrt(s / (W)a.n + (W)a.eps);
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+         const int64_t i = chunk_first<true>(v, threads, t);
+         if (a.h.p != nullptr) put<T, true>(a.h, row, i, a.n, h[v]);
+#pragma unroll
+         for (int j = 0; j < 8; j++) h[v][j] = h[v][j] * rr * to_acc(w[v].e[j]);
+         if (QUANT) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = i < a.n ? (float)h[v][j] : 0.0f;
+            put_codes<true>(a, row, i, f, lane, 0xFFFFFFFFu);
+         } else put<T, true>(a.y, row, i, a.n, h[v]);
+      }
+   }
+   if (!ring.ok && t == 0) for (int k = max(0, it - stages); k < it; k++) tc::bar_wait(ring.bars + 8 * (k % stages), (k / stages) & 1);
+}
+
 // Rows too long for the registers of a block: the block reads the row twice (the second time from the L2 cache).  h is
 // written in the second pass, each element by the thread that has just read it, so that h may stand in place of x or
 // of the residual.
@@ -301,7 +403,7 @@ __global__ void __launch_bounds__(MAXT) grad_rows(const __grid_constant__ GradAr
          }
       Eight<T> cg[V], ch[V], cr[V];
 #pragma unroll
-      for (int v = 0; v < V; v++) { cg[v] = g[v]; ch[v] = h[v]; cr[v] = r[v]; }
+      for (int v = 0; v < V; v++) { cg[v] = g[v]; ch[v] = h[v]; if (has_res) cr[v] = r[v]; }
       if (PIPE && row + step < a.rows) fetch_row(row + step);
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) if (BLOCK || d < group) { s += __shfl_xor_sync(mask, s, d); p += __shfl_xor_sync(mask, p, d); }
@@ -354,6 +456,102 @@ __global__ void __launch_bounds__(MAXT) grad_rows(const __grid_constant__ GradAr
          __syncthreads();
       }
       for (int64_t k = threadIdx.x; k < a.n; k += blockDim.x) part[k] = join[k];
+   }
+}
+
+template <class T, int V, int MAXT>
+__global__ void __launch_bounds__(MAXT) grad_ring(const __grid_constant__ GradArgs a, int stages)
+{
+   using W = typename Real<T>::acc;
+   extern __shared__ __align__(128) char smem[];
+   __shared__ alignas(8) uint64_t bar[RING_MAX];
+   __shared__ W sums[2][2][32];
+   const int lane = threadIdx.x & 31, t = threadIdx.x, threads = blockDim.x;
+   const bool has_res = a.res.p != nullptr;
+   const int bytes = (int)(a.n * sizeof(T));
+   Ring ring;
+   ring.start(smem, bar, (has_res ? 3 : 2) * bytes, stages);
+   auto load = [&](int it) {
+      const int64_t row = blockIdx.x + (int64_t)it * gridDim.x;
+      if (row >= a.rows) return;
+      const int s = it % stages;
+      tc::bar_expect(ring.bars + 8 * s, ring.stage);
+      ring.copy(s, 0, a.dy, row, bytes);
+      ring.copy(s, bytes, a.h, row, bytes);
+      if (has_res) ring.copy(s, 2 * bytes, a.res, row, bytes);
+   };
+   if (t == 0) for (int it = 0; it < stages; it++) load(it);
+   Eight<T> w[V];
+   W dw[V][8];
+#pragma unroll
+   for (int v = 0; v < V; v++) {
+      fetch_weights<T, true>(w[v], a.w, chunk_first<true>(v, threads, t), a.n);
+#pragma unroll
+      for (int j = 0; j < 8; j++) dw[v][j] = 0;
+   }
+   const W inv_n = (W)1 / (W)a.n;
+   int it = 0;
+   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, it++) {
+      ring.wait(it);
+      const char *place = smem + (it % stages) * ring.stage;
+      W s = 0, p = 0;
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+         const int i = (v * threads + t) * 8;
+         if (i < a.n) {
+            const Eight<T> g = load_eight<T>(place + i * sizeof(T)), h = load_eight<T>(place + bytes + i * sizeof(T));
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+               const W hv = to_acc(h.e[j]);
+               s = fma(hv, hv, s);
+               p = fma(to_acc(g.e[j]) * to_acc(w[v].e[j]), hv, p);
+            }
+         }
+      }
+      if (!ring.ok) s = (W)NAN;
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) { s += __shfl_xor_sync(0xFFFFFFFFu, s, d); p += __shfl_xor_sync(0xFFFFFFFFu, p, d); }
+      if (lane == 0) { sums[it & 1][0][t >> 5] = s; sums[it & 1][1][t >> 5] = p; }
+      __syncthreads();
+      if (t == 0 && it > 0) load(it - 1 + stages);
+      s = 0; p = 0;
+      for (int k = 0; k < threads / 32; k++) { s += sums[it & 1][0][k]; p += sums[it & 1][1][k]; }
+      const W rr = (W)1 / sqrt(s / (W)a.n + (W)a.eps);
+      const W c = rr * rr * rr * (p * inv_n);
+#pragma unroll
+      for (int v = 0; v < V; v++) {                       // the row once more from shared memory: no registers between
+         const int i = (v * threads + t) * 8;
+         if (i < a.n) {
+            const Eight<T> g = load_eight<T>(place + i * sizeof(T)), h = load_eight<T>(place + bytes + i * sizeof(T));
+            W d[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+               const W gv = to_acc(g.e[j]), hv = to_acc(h.e[j]);
+               d[j] = fma(rr, gv * to_acc(w[v].e[j]), -hv * c);
+               dw[v][j] = fma(gv, hv * rr, dw[v][j]);
+            }
+            if (has_res) {
+               const Eight<T> r = load_eight<T>(place + 2 * bytes + i * sizeof(T));
+#pragma unroll
+               for (int j = 0; j < 8; j++) d[j] += to_acc(r.e[j]);
+            }
+            put<T, true>(a.dh, row, i, a.n, d);
+         }
+      }
+   }
+   if (!ring.ok && t == 0) for (int k = max(0, it - stages); k < it; k++) tc::bar_wait(ring.bars + 8 * (k % stages), (k / stages) & 1);
+   if (a.part != nullptr) {
+      W *part = (W *)a.part + (int64_t)blockIdx.x * a.n;
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+         const int i = (v * threads + t) * 8;
+         if (i < a.n) {
+            Eight<W> o;
+#pragma unroll
+            for (int j = 0; j < 8; j++) o.e[j] = dw[v][j];
+            store_eight(part + i, o);
+         }
+      }
    }
 }
 
@@ -489,6 +687,29 @@ static int launch_norm(NormArgs &a, int threads, int sms, cudaStream_t stream)
    return 0;
 }
 
+// Shared memory of an SM, shared by as many blocks as keep 1024 threads or so on it
+struct RingPlan { int per_sm, stages; size_t smem; };
+static RingPlan ring_plan(int64_t stage_bytes, int threads)
+{
+   RingPlan p;
+   for (p.per_sm = std::min(4, std::max(1, 1024 / threads)); p.per_sm >= 1; p.per_sm--) {
+      p.stages = (int)std::min<int64_t>(RING_MAX, (225 * 1024 / p.per_sm - 2048) / stage_bytes);
+      if (p.stages >= 3 || (p.per_sm == 1 && p.stages == 2)) break;
+   }
+   p.smem = p.per_sm >= 1 ? (size_t)(p.stages * stage_bytes) : 0;
+   return p;
+}
+
+template <class T, int V, bool QUANT>
+static int launch_norm_ring(NormArgs &a, const RingPlan &p, int threads, int sms, cudaStream_t stream)
+{
+   auto *kernel = norm_ring<T, V, QUANT, 512>;
+   SD_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem));
+   kernel<<<(unsigned)std::min<int64_t>(a.rows, (int64_t)p.per_sm * sms), threads, p.smem, stream>>>(a, p.stages);
+   SD_LAUNCH_CHECK();
+   return 0;
+}
+
 template <class T, bool VEC, bool QUANT>
 static int norm_of(NormArgs &a, cudaStream_t stream)
 {
@@ -500,9 +721,17 @@ static int norm_of(NormArgs &a, cudaStream_t stream)
    a.group = VEC && n <= 128 ? 16 : 32;
    if (n <= 256)  return launch_norm<T, 1, false, VEC, true, QUANT, 256>(a, 256, sms, stream);
    if (n <= 512)  return launch_norm<T, 2, false, VEC, true, QUANT, 256>(a, 256, sms, stream);
-   if (n <= 1024) return launch_norm<T, 4, false, VEC, !WIDE, QUANT, 256>(a, 256, sms, stream);
    // few rows: a thread takes eight elements, so that a row is one round of loads
    if (a.rows <= sms && n <= 8192) return launch_norm<T, 1, true, VEC, false, QUANT, 1024>(a, round32(eights), sms, stream);
+   if constexpr (VEC) {
+      if (n <= NORM_MAX) {
+         const int threads = std::max(64, round32((eights + (n <= 8192 ? 1 : 3)) / (n <= 8192 ? 2 : 4)));
+         const RingPlan p = ring_plan(n * (int64_t)sizeof(T) * (a.res.p != nullptr ? 2 : 1), threads);
+         if (p.per_sm >= 1) return n <= 8192 ? launch_norm_ring<T, 2, QUANT>(a, p, threads, sms, stream)
+                                             : launch_norm_ring<T, 4, QUANT>(a, p, threads, sms, stream);
+      }
+   }
+   if (n <= 1024) return launch_norm<T, 4, false, VEC, !WIDE, QUANT, 256>(a, 256, sms, stream);
    if (n <= 2048) return launch_norm<T, 1, true, VEC, true, QUANT, 256>(a, round32(eights), sms, stream);
    if (n <= 8192) return launch_norm<T, 2, true, VEC, !WIDE, QUANT, 512>(a, round32((eights + 1) / 2), sms, stream);
    if constexpr (!WIDE) {
@@ -551,7 +780,8 @@ static int fill_norm(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x
 }
 
 // ---- gradient ----
-struct GradPlan { int kind, threads, blocks; };           // kind: 1, 2, 4 eights a warp's thread; 11, 12, 14 a block's; 20 long
+// kind: 1, 2 eights of a warp's thread; 11, 12, 14 of a block's; 20 long rows
+struct GradPlan { int kind, threads, blocks; };
 
 template <class T> static bool grad_vec(const GradArgs &a)
 {
@@ -567,35 +797,57 @@ static GradPlan grad_plan(int64_t n, int64_t rows, size_t elemsize, int sms)
    const bool wide = elemsize == 8;
    const int64_t eights = (n + 7) / 8;
    GradPlan p;
-   if (n <= 1024)      { p.kind = n <= 256 ? 1 : n <= 512 ? 2 : 4; p.threads = 256; }
-   else if (n <= 2048) { p.kind = 11; p.threads = round32(eights); }
+   if (n <= 512)       { p.kind = n <= 256 ? 1 : 2; p.threads = 256; }
+   else if (n <= 1024) { p.kind = 11; p.threads = round32(eights); }
    else if (n <= 8192) { p.kind = 12; p.threads = round32((eights + 1) / 2); }
    else if (n <= NORM_MAX && !wide) { p.kind = 14; p.threads = round32((eights + 3) / 4); }
    else                { p.kind = 20; p.threads = 256; }
    const int64_t rows_at_once = p.kind < 10 ? 8 : 1;      // warps of a block
-   int64_t most = p.kind == 20 ? 16 : p.kind == 14 ? sms : (int64_t)sms * std::max(1, 512 / p.threads);
+   const int64_t most = p.kind == 20 ? 16 : (int64_t)sms * std::min(4, std::max(1, 512 / p.threads));
    const int64_t want = (rows + rows_at_once - 1) / rows_at_once;
    p.blocks = (int)std::max<int64_t>(1, std::min(want, most));
    return p;
 }
 
 template <class T, int V, bool BLOCK, bool VEC, bool PIPE, int MAXT>
-static void launch_grad(GradArgs &a, const GradPlan &p, cudaStream_t stream)
+static int launch_grad(GradArgs &a, const GradPlan &p, cudaStream_t stream)
 {
    const size_t smem = BLOCK ? 0 : (size_t)a.n * sizeof(typename Real<T>::acc);
    grad_rows<T, V, BLOCK, VEC, PIPE, MAXT><<<p.blocks, p.threads, smem, stream>>>(a);
+   SD_LAUNCH_CHECK();
+   return 0;
 }
 
-template <class T, bool VEC> static void grad_of(GradArgs &a, const GradPlan &p, cudaStream_t stream)
+template <class T, int V> static int launch_grad_ring(GradArgs &a, const GradPlan &p, int stages, size_t smem, cudaStream_t stream)
+{
+   auto *kernel = grad_ring<T, V, 512>;
+   SD_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+   kernel<<<p.blocks, p.threads, smem, stream>>>(a, stages);
+   SD_LAUNCH_CHECK();
+   return 0;
+}
+
+template <class T, bool VEC> static int grad_of(GradArgs &a, const GradPlan &p, int sms, cudaStream_t stream)
 {
    constexpr bool WIDE = sizeof(T) == 8;
    a.group = 32;
-   if (p.kind == 1)       launch_grad<T, 1, false, VEC, true, 256>(a, p, stream);
-   else if (p.kind == 2)  launch_grad<T, 2, false, VEC, !WIDE, 256>(a, p, stream);
-   else if (p.kind == 4)  launch_grad<T, 4, false, VEC, false, 256>(a, p, stream);
-   else if (p.kind == 11) launch_grad<T, 1, true, VEC, true, 256>(a, p, stream);
-   else if (p.kind == 12) launch_grad<T, 2, true, VEC, sizeof(T) == 2, 512>(a, p, stream);
-   else if constexpr (!WIDE) launch_grad<T, 4, true, VEC, false, 512>(a, p, stream);
+   if (p.kind == 1) return launch_grad<T, 1, false, VEC, true, 256>(a, p, stream);
+   if (p.kind == 2) return launch_grad<T, 2, false, VEC, !WIDE, 256>(a, p, stream);
+   if constexpr (VEC) {
+      const int per_sm = (p.blocks + sms - 1) / sms;
+      const int64_t stage = a.n * (int64_t)sizeof(T) * (a.res.p != nullptr ? 3 : 2);
+      const int stages = (int)std::min<int64_t>(RING_MAX, (225 * 1024 / per_sm - 2048) / stage);
+      if (stages >= 2) {
+         const size_t smem = (size_t)(stages * stage);
+         if (p.kind == 11) return launch_grad_ring<T, 1>(a, p, stages, smem, stream);
+         if (p.kind == 12) return launch_grad_ring<T, 2>(a, p, stages, smem, stream);
+         if constexpr (!WIDE) return launch_grad_ring<T, 4>(a, p, stages, smem, stream);
+      }
+   }
+   if (p.kind == 11) return launch_grad<T, 1, true, VEC, false, 256>(a, p, stream);
+   if (p.kind == 12) return launch_grad<T, 2, true, VEC, false, 512>(a, p, stream);
+   if constexpr (!WIDE) return launch_grad<T, 4, true, VEC, false, 512>(a, p, stream);
+   return 0;
 }
 
 template <class T> static int grad_typed(GradArgs &a, void *dw, void *buffer, cudaStream_t stream)
@@ -612,8 +864,7 @@ template <class T> static int grad_typed(GradArgs &a, void *dw, void *buffer, cu
       SD_LAUNCH_CHECK();
       grad_long_apply<T><<<dim3((unsigned)((a.n + 2047) / 2048), (unsigned)p.blocks), 256, 0, stream>>>(a, rowsums);
    }
-   else if (grad_vec<T>(a)) grad_of<T, true>(a, p, stream);
-   else grad_of<T, false>(a, p, stream);
+   else if ((grad_vec<T>(a) ? grad_of<T, true>(a, p, dev.sms, stream) : grad_of<T, false>(a, p, dev.sms, stream)) != 0) return -1;
    SD_LAUNCH_CHECK();
    if (dw != nullptr) {
       grad_join<W><<<(unsigned)((a.n + 31) / 32), 256, 0, stream>>>(part, p.blocks, a.n, (W *)dw);
