@@ -534,6 +534,24 @@ def _row_input(x: Tensor, what: str):
     return _row_operand(x, x.dtype, x.size, x.storage.device, "the input")
 
 
+def _view(storage, dtype: str, size, strides, offset: int = 0) -> Tensor:
+    """A tensor of fields that are known to be right."""
+    t = Tensor.__new__(Tensor)
+    t.storage, t.dtype, t.size, t.strides, t.offset, t.byteswapped = storage, dtype, size, strides, offset, False
+    return t
+
+
+def _new(storage, size, dtype: str):
+    """A new column-major tensor beside `storage`, and its Matrix."""
+    es = dt.SIZE[dtype]
+    strides, step = [], es
+    for s in size:
+        strides.append(step)
+        step *= s
+    t = _view(storage.new_empty(step if step > 16 else 16), dtype, list(size), strides)
+    return t, _lib.Matrix(t.storage.data_ptr(), es, es * size[0])
+
+
 def _norm_weight(weight, x: Tensor):
     """The weights as the kernels take them (contiguous, in the type of x) and their address."""
     if weight is None:
@@ -542,27 +560,27 @@ def _norm_weight(weight, x: Tensor):
         raise ValueError("the weights need size [%d]" % x.size[0])
     if weight.storage.device != x.storage.device:
         raise ValueError("weight is on another device")
-    w = _prepared(weight, x.dtype, weight.size)
-    if w.size[0] > 1 and w.strides[0] != w.elemsize:
-        w = clone(w)
-    return w, w.storage.data_ptr() + w.offset
+    es = dt.SIZE[x.dtype]
+    p = weight.storage.data_ptr() + weight.offset
+    if weight.dtype == x.dtype and weight.strides[0] == es and not weight.byteswapped and p % es == 0:
+        return weight, p
+    w = clone(_prepared(weight, x.dtype, weight.size))
+    return w, w.storage.data_ptr()
 
 
-def _result(dst, size, dtype: str, device):
+def _result(dst, size, dtype: str, storage):
     """Where a kernel writes, and its Matrix: dst itself where the kernel can, else a new tensor that is copied there."""
     if dst is not None:
         if dst.size != size:
             raise ValueError("the result has size %s, not %s" % (size, dst.size))
-        if dst.storage.device != device:
+        if dst.storage.device != storage.device:
             raise ValueError("the result is on another device")
         r = _as_rows(dst)
         if dst.dtype == dtype and not dst.byteswapped and r is not None and \
                 dst.ptr % dst.elemsize == 0 and _py.all(s % dst.elemsize == 0 for s in dst.strides) and \
                 _py.all(st != 0 or s <= 1 for s, st in zip(dst.size, dst.strides)):
             return dst, _lib.Matrix(dst.ptr, dst.strides[0], r[1])
-    out = Tensor.empty(size, dtype, device)
-    es = dt.SIZE[dtype]
-    return out, _lib.Matrix(out.storage.data_ptr(), es, es * size[0])
+    return _new(storage, size, dtype)
 
 
 def _delivered(out: Tensor, dst) -> Tensor:
@@ -584,9 +602,8 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residua
     With a residual the sum h = x + residual is normalised (before it is rounded) and returned too: (y, h).  dst and h
     say where y and h go; h may be the residual's own tensor, dst that of x."""
     x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, "rms_norm")
-    device = x.storage.device
-    out, my = _result(dst, x.size, x.dtype, device)
-    lib, stream = _here(device)
+    out, my = _result(dst, x.size, x.dtype, x.storage)
+    lib, stream = _here(x.storage.device)
     lib.rms_norm(x.dtype, x.size[0], rows, mx, mr, pw, eps, mh, my, stream)
     y = _delivered(out, dst)
     return y if total is None else (y, _delivered(total, h))
@@ -600,21 +617,19 @@ def _norm_operands(x, weight, residual, h, what):
         if h is not None:
             raise ValueError("h is x + residual: there is no residual")
         return x, rows, mx, None, None, w, pw, None, None
-    device = x.storage.device
-    res, _, mr = _row_operand(residual, x.dtype, x.size, device, "residual")
-    total, mh = _result(h, x.size, x.dtype, device)
+    res, _, mr = _row_operand(residual, x.dtype, x.size, x.storage.device, "residual")
+    total, mh = _result(h, x.size, x.dtype, x.storage)
     return x, rows, mx, res, mr, w, pw, total, mh
 
 
-def _empty_blocks(n: int, rows: int, block: int, format: str, device):
-    """Room for codes (rows padded to 16 bytes) and scales, and its BlocksView."""
+def _empty_blocks(n: int, rows: int, block: int, format: str, storage):
+    """Room for codes (rows padded to 16 bytes) with the scales behind them, and its BlocksView."""
     ld = (n + 15) // 16 * 16
-    rb = (rows + block - 1) // block
-    codes = Tensor.empty([ld, rows], "uint8", device)
-    codes.size[0] = n
-    scales = Tensor.empty([rb, (n + 127) // 128], "float", device)
-    return Blocks(codes, scales, format), _lib.BlocksView(codes.storage.data_ptr(), ld, scales.storage.data_ptr(), 4, 4 * rb,
-                                                          block, _lib.FORMATS[format])
+    rb, nb = (rows + block - 1) // block, (n + 127) // 128
+    room = storage.new_empty(ld * rows + 4 * rb * nb // 16 * 16 + 16)
+    p = room.data_ptr()
+    return Blocks(_view(room, "uint8", [n, rows], [1, ld]), _view(room, "float", [rb, nb], [4, 4 * rb], ld * rows), format), \
+        _lib.BlocksView(p, ld, p + ld * rows, 4, 4 * rb, block, _lib.FORMATS[format])
 
 
 def _blocks_view(b: Blocks, what: str):
@@ -646,9 +661,8 @@ def rms_norm_quantize(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6
     """rms_norm whose y is returned as Blocks, a scale for 128 elements of each row; with a residual (Blocks, h)."""
     _format(format)
     x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, "rms_norm_quantize")
-    device = x.storage.device
-    out, view = _empty_blocks(x.size[0], rows, 1, format, device)
-    lib, stream = _here(device)
+    out, view = _empty_blocks(x.size[0], rows, 1, format, x.storage)
+    lib, stream = _here(x.storage.device)
     lib.rms_norm_quantize(x.dtype, x.size[0], rows, mx, mr, pw, eps, mh, view, stream)
     return out if total is None else (out, _delivered(total, h))
 
@@ -658,7 +672,6 @@ def rms_norm_grad(dy: Tensor, h: Tensor, weight: Tensor | None = None, eps: floa
     """Gradient of rms_norm at h (the input, or x + residual): returns (dh, dweight).
 
     dres, the gradient that reaches h past the norm, is added to dh.  dweight is in the work type (half: float)."""
-    import torch
     h, rows, mh = _row_input(h, "rms_norm_grad")
     if dy.size != h.size or (dres is not None and dres.size != h.size):
         raise ValueError("gradients have the size of h, %s" % h.size)
@@ -668,12 +681,12 @@ def rms_norm_grad(dy: Tensor, h: Tensor, weight: Tensor | None = None, eps: floa
     mr = None
     if dres is not None:
         dres, _, mr = _row_operand(dres, dtype, h.size, device, "dres")
-    out, mo = _result(dst, h.size, dtype, device)
-    dweight = Tensor.empty([n], "double" if dtype == "double" else "float", device)
+    out, mo = _result(dst, h.size, dtype, h.storage)
+    dweight, md = _new(h.storage, [n], "double" if dtype == "double" else "float")
     lib, stream = _here(device)
     # a buffer of its own for each call: calls on several streams and captured graphs share nothing
-    buf = torch.empty(lib.rms_norm_grad_buffer_size(dtype, n, rows, device.index) + 16, dtype=torch.uint8, device=device)
-    lib.rms_norm_grad(dtype, n, rows, mg, mh, pw, eps, mr, mo, dweight.storage.data_ptr(), buf.data_ptr(), stream)
+    buf = h.storage.new_empty(lib.rms_norm_grad_buffer_size(dtype, n, rows, device.index) + 16)
+    lib.rms_norm_grad(dtype, n, rows, mg, mh, pw, eps, mr, mo, md.ptr, buf.data_ptr(), stream)
     return _delivered(out, dst), dweight
 
 
@@ -686,9 +699,8 @@ def block_quantize(x: Tensor, block: int = 1, format: str = "e4m3") -> Blocks:
     if block not in (1, 128):
         raise ValueError("a scale belongs to 1 or 128 rows")
     x, rows, mx = _row_input(x, "block_quantize")
-    device = x.storage.device
-    out, view = _empty_blocks(x.size[0], rows, block, format, device)
-    lib, stream = _here(device)
+    out, view = _empty_blocks(x.size[0], rows, block, format, x.storage)
+    lib, stream = _here(x.storage.device)
     lib.block_quantize(x.dtype, x.size[0], rows, mx, view, stream)
     return out
 
@@ -710,7 +722,7 @@ def block_gemm(a: Blocks, b: Blocks, dtype: str = "half", dst: Tensor | None = N
     if kb.storage.device != device:
         raise ValueError("block_gemm: operands on different devices")
     n = kb.size[1]
-    out, mc = _result(dst, [m, n], dtype, device)
+    out, mc = _result(dst, [m, n], dtype, ka.storage)
     lib, stream = _here(device)
     lib.block_gemm(dtype, m, n, k, va, vb, mc, stream)
     return _delivered(out, dst)
