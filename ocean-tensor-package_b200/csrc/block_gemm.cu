@@ -100,208 +100,260 @@ __global__ void __launch_bounds__(256) gemm_plain(const __grid_constant__ GemmAr
 constexpr int BM = 128;
 constexpr int TILE_P = BM * B8_BLOCK;                     // bytes of a stage's 128 rows
 
-template <int BN> struct Shape {
+constexpr int AHEAD = 4;                                  // depth blocks whose scales are under way
+
+// PAIR: two blocks share a tile of 256 rows, each holds half of either operand's rows; the columns' half travels once
+// instead of twice, and the 64 bytes a cycle that a block can take in no longer bound the products.
+template <int BN, bool PAIR> struct Shape {
    static constexpr int groups = BN > 128 ? 2 : 1;        // epilogue warpgroups, 128 columns at most each
    static constexpr int columns = BN / groups;
-   static constexpr int threads = groups * 128 + 64;      // and a warp that loads, a warp that multiplies
-   static constexpr int stage = TILE_P + BN * B8_BLOCK;
+   static constexpr int run = columns >= 64 ? 32 : columns / 2;     // columns of one read of tensor memory
+   // and a warp that loads, a warp that multiplies; with two groups a third whole one, so that registers can be moved:
+   // 384 x 168 = 128 x 40 + 256 x 232
+   static constexpr int threads = groups == 2 ? 384 : groups * 128 + 64;
+   static constexpr int rows_q = PAIR ? BN / 2 : BN;      // of q in this block's shared memory
+   static constexpr int stage = TILE_P + rows_q * B8_BLOCK;
    static constexpr int resident = BN >= 128 ? 1 : 2;     // blocks an SM: one whose ring fills shared memory, or two
-   static constexpr int stages = BN == 256 ? 4 : BN == 128 ? 6 : BN == 64 ? 4 : BN == 32 ? 5 : 6;
+   static constexpr int stages = PAIR || BN != 64 ? 5 : 4;
    static constexpr int tmem = 2 * BN < 32 ? 32 : 2 * BN;
-   static constexpr int scales = 2 * BN * 4;              // two blocks' scales of the columns
-   static constexpr int smem = 1024 + stages * stage + scales;
+   static constexpr int scales = 2 * AHEAD * groups * 128 * 4;      // a row's and a column's for each epilogue thread
+   static constexpr int out = BN >= 128 ? groups * 4 * 4096 : 0;    // 32 rows of 128 bytes for each epilogue warp
+   static constexpr int smem = 1024 + stages * stage + scales + out;
 };
+
+// A warp's 32 rows of results, a thread each, to memory where a row's results lie side by side: 128 bytes of every row
+// at a time through shared memory, so that a store writes whole lines.  Places of 16 bytes are permuted by the row.
+template <int CW, bool HALF>
+__device__ __forceinline__ void store_rows(const GemmArgs &a, const float (&acc)[CW], char *buf, int64_t p0, int64_t q0, int lane)
+{
+   constexpr int PER = HALF ? 64 : 32, UNIT = PER / 8;    // results in 128 bytes, in 16
+#pragma unroll
+   for (int c = 0; c < CW; c += PER) {
+      if (PER > CW) break;
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+         uint4 w;
+         if (HALF) {
+            uint32_t x[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+               const __half2 h = __floats2half2_rn(acc[c + 8 * u + 2 * k], acc[c + 8 * u + 2 * k + 1]);
+               x[k] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+            w = make_uint4(x[0], x[1], x[2], x[3]);
+         } else w = make_uint4(__float_as_uint(acc[c + 4 * u]), __float_as_uint(acc[c + 4 * u + 1]), __float_as_uint(acc[c + 4 * u + 2]), __float_as_uint(acc[c + 4 * u + 3]));
+         *reinterpret_cast<uint4 *>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = w;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int r = 0; r < 8; r++) {
+         const int row = 4 * r + (lane >> 3), u = lane & 7;
+         const uint4 w = *reinterpret_cast<const uint4 *>(buf + row * 128 + ((u ^ (row & 7)) << 4));
+         const int64_t p = p0 + row, q = q0 + c + u * UNIT;
+         char *d = a.c + p * a.cp + q * (HALF ? 2 : 4);
+         if (p < a.p.rows) {
+            if (q + UNIT <= a.q.rows) *reinterpret_cast<uint4 *>(d) = w;
+            else {
+               const uint32_t x[4] = { w.x, w.y, w.z, w.w };
+#pragma unroll
+               for (int k = 0; k < UNIT; k++) {
+                  if (q + k >= a.q.rows) continue;
+                  if (HALF) reinterpret_cast<uint16_t *>(d)[k] = (uint16_t)(x[k >> 1] >> (16 * (k & 1)));
+                  else      reinterpret_cast<uint32_t *>(d)[k] = x[k];
+               }
+            }
+         }
+      }
+   }
+}
 
 // COLVEC: a scale for every row of q (a vector over the columns); otherwise for 128 rows (one number).
 // SPLIT: a cluster shares the tile, block r takes the r-th part of the depth.
-template <int BN, bool COLVEC, bool SPLIT>
-__global__ void __launch_bounds__(Shape<BN>::threads, Shape<BN>::resident)
+template <int BN, bool PAIR, bool COLVEC, bool SPLIT>
+__global__ void __launch_bounds__(Shape<BN, PAIR>::threads, Shape<BN, PAIR>::resident)
 gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ GemmArgs a,
            int splits, int kblocks, int ptiles, int qtiles)
 {
-   using S = Shape<BN>;
+   using S = Shape<BN, PAIR>;
    constexpr int ST = S::stages, CW = S::columns;
    extern __shared__ char raw[];
    __shared__ alignas(8) uint64_t bars[2 * ST + 4];
    __shared__ uint32_t tmem_base;
    __shared__ int failed;
    char *ring = raw + ((1024 - (tc::smem_u32(raw) & 1023)) & 1023);
-   float *colscale = (float *)(ring + ST * S::stage);     // [2][BN]
+   float *scales = (float *)(ring + ST * S::stage);       // [AHEAD][groups * 128] of rows, the same of columns
+   char *out = ring + ST * S::stage + S::scales;
    const uint32_t ring_u = tc::smem_u32(ring);
    const uint32_t full = tc::smem_u32(bars), empty = full + 8 * ST, tfull = full + 16 * ST, tempty = tfull + 16;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
    constexpr int EPI = S::groups * 4;                     // epilogue warps come first: warp w reads lanes 32 (w % 4)
+   const int rank = PAIR || SPLIT ? (int)tc::cluster_rank() : 0;
+   const bool leader = !PAIR || rank == 0;
 
    if (threadIdx.x == 0) {
       for (int s = 0; s < ST; s++) { tc::bar_init(full + 8 * s, 1); tc::bar_init(empty + 8 * s, 1); }
-      for (int b = 0; b < 2; b++) { tc::bar_init(tfull + 8 * b, 1); tc::bar_init(tempty + 8 * b, EPI); }
+      for (int b = 0; b < 2; b++) { tc::bar_init(tfull + 8 * b, 1); tc::bar_init(tempty + 8 * b, PAIR ? 2 * EPI : EPI); }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       failed = 0;
    }
-   if (warp == EPI) tc::alloc(tc::smem_u32(&tmem_base), S::tmem);
+   if (warp == EPI) tc::alloc<PAIR>(tc::smem_u32(&tmem_base), S::tmem);
    tc::fence_before();
    __syncthreads();
+   if (PAIR) tc::cluster_sync();
    tc::fence_after();
    const uint32_t tmem = *(volatile uint32_t *)&tmem_base;
 
+   // ptiles counts tiles of 128 rows, or of 256 for pairs
    const int ntiles = ptiles * qtiles;
-   const int rank = SPLIT ? (int)tc::cluster_rank() : 0;
-   const int first = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x, step = SPLIT ? ntiles : (int)gridDim.x;
+   const int first = SPLIT ? (int)blockIdx.x / splits : PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x;
+   const int step = SPLIT ? ntiles : PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
    const int kb0 = SPLIT ? (int)((long long)kblocks * rank / splits) : 0;
    const int kb1 = SPLIT ? (int)((long long)kblocks * (rank + 1) / splits) : kblocks;
-   // Tiles in panels of 16 rows of tiles, so that blocks at work share both operands in the L2 cache
+   constexpr int ROWS = PAIR ? 2 * BM : BM;
+   const int prow = PAIR ? rank * BM : 0, qrow = PAIR ? rank * S::rows_q : 0;
+   // Tiles in panels of `ROWS` times 16 or 8 rows, so that blocks at work share both operands in the L2 cache
    auto place = [&](int tile, int &tp, int &tq) {
-      const int panel = tile / (16 * qtiles), rest = tile - panel * 16 * qtiles;
-      const int height = min(16, ptiles - panel * 16);
-      tp = panel * 16 + rest % height; tq = rest / height;
+      constexpr int PANEL = PAIR ? 8 : 16;
+      const int panel = tile / (PANEL * qtiles), rest = tile - panel * PANEL * qtiles;
+      const int height = min(PANEL, ptiles - panel * PANEL);
+      tp = panel * PANEL + rest % height; tq = rest / height;
    };
 
-   if (warp == EPI && lane == 0) {                        // ---- loads
-      int it = 0; bool ok = true;
-      for (int tile = first; tile < ntiles && ok; tile += step) {
-         int tp, tq; place(tile, tp, tq);
-         for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int s = it % ST;
-            if (it >= ST && !tc::bar_wait(empty + 8 * s, (it / ST - 1) & 1)) { ok = false; break; }
-            const uint32_t dst = ring_u + s * S::stage;
-            tc::bar_expect(full + 8 * s, S::stage);
-            tc::load_box(dst, &map_p, full + 8 * s, kb * B8_BLOCK, tp * BM);
-            tc::load_box(dst + TILE_P, &map_q, full + 8 * s, kb * B8_BLOCK, tq * BN);
+   if (warp >= EPI) {
+      if (S::groups == 2) tc::registers_down<40>();
+      if (warp == EPI && lane == 0) {                     // ---- loads
+         const uint32_t full_at = PAIR ? tc::at_rank(full, 0) : full;
+         int it = 0; bool ok = true;
+         for (int tile = first; tile < ntiles && ok; tile += step) {
+            int tp, tq; place(tile, tp, tq);
+            for (int kb = kb0; kb < kb1; kb++, it++) {
+               const int s = it % ST;
+               if (it >= ST && !tc::bar_wait(empty + 8 * s, (it / ST - 1) & 1)) { ok = false; break; }
+               const uint32_t dst = ring_u + s * S::stage;
+               if (leader) tc::bar_expect(full + 8 * s, PAIR ? 2 * S::stage : S::stage);
+               tc::load_box<PAIR>(dst, &map_p, full_at + 8 * s, kb * B8_BLOCK, tp * ROWS + prow);
+               tc::load_box<PAIR>(dst + TILE_P, &map_q, full_at + 8 * s, kb * B8_BLOCK, tq * BN + qrow);
+            }
          }
-      }
-      if (!ok) {                                          // the copies under way end before shared memory is given back
-         *(volatile int *)&failed = 1;
-         for (int k = max(0, it - ST); k < it; k++) tc::bar_wait(full + 8 * (k % ST), (k / ST) & 1);
-      }
-   } else if (warp == EPI + 1 && lane == 0) {             // ---- products
-      const uint32_t idesc = (1u << 4) | ((uint32_t)a.p.format << 7) | ((uint32_t)a.q.format << 10) | ((uint32_t)(BN / 8) << 17) | ((uint32_t)(BM / 16) << 24);
-      int it = 0; bool ok = true;
-      for (int tile = first; tile < ntiles && ok; tile += step)
-         for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int s = it % ST, b = it & 1;
-            if (it >= 2 && !tc::bar_wait(tempty + 8 * b, (it / 2 - 1) & 1)) { ok = false; break; }
-            if (!tc::bar_wait(full + 8 * s, (it / ST) & 1)) { ok = false; break; }
-            tc::fence_after();
-            const uint64_t dp = tc::tile_descriptor(ring_u + s * S::stage), dq = tc::tile_descriptor(ring_u + s * S::stage + TILE_P);
+         if (!ok) {                                       // the copies under way end before shared memory is given back
+            *(volatile int *)&failed = 1;
+            if (leader) for (int k = max(0, it - ST); k < it; k++) tc::bar_wait(full + 8 * (k % ST), (k / ST) & 1);
+         }
+      } else if (warp == EPI + 1 && lane == 0 && leader) {   // ---- products
+         const uint32_t idesc = (1u << 4) | ((uint32_t)a.p.format << 7) | ((uint32_t)a.q.format << 10) | ((uint32_t)(BN / 8) << 17) | ((uint32_t)(ROWS / 16) << 24);
+         int it = 0; bool ok = true;
+         for (int tile = first; tile < ntiles && ok; tile += step)
+            for (int kb = kb0; kb < kb1; kb++, it++) {
+               const int s = it % ST, b = it & 1;
+               if (it >= 2 && !tc::bar_wait(tempty + 8 * b, (it / 2 - 1) & 1)) { ok = false; break; }
+               if (!tc::bar_wait(full + 8 * s, (it / ST) & 1)) { ok = false; break; }
+               tc::fence_after();
+               const uint64_t dp = tc::tile_descriptor(ring_u + s * S::stage), dq = tc::tile_descriptor(ring_u + s * S::stage + TILE_P);
 #pragma unroll
-            for (int k = 0; k < 4; k++) tc::mma_f8(tmem + b * BN, dp + 2 * k, dq + 2 * k, idesc, k > 0);
-            tc::commit(empty + 8 * s);
-            tc::commit(tfull + 8 * b);
+               for (int k = 0; k < 4; k++) tc::mma_f8<PAIR>(tmem + b * BN, dp + 2 * k, dq + 2 * k, idesc, k > 0);
+               tc::commit<PAIR>(empty + 8 * s);
+               tc::commit<PAIR>(tfull + 8 * b);
+            }
+         if (!ok) {
+            *(volatile int *)&failed = 1;
+            if (it > 0) tc::bar_wait(tfull + 8 * ((it - 1) & 1), ((it - 1) / 2) & 1);
          }
-      if (!ok) {
-         *(volatile int *)&failed = 1;
-         if (it > 0) tc::bar_wait(tfull + 8 * ((it - 1) & 1), ((it - 1) / 2) & 1);
       }
-   } else if (warp < EPI) {                               // ---- scales and sums
+   } else {                                               // ---- scales and sums
+      if (S::groups == 2) tc::registers_up<232>();
       const int group = warp >> 2, row = (warp & 3) * 32 + lane, col0 = group * CW;
       const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + col0;
+      const uint32_t tempty_at = PAIR ? tc::at_rank(tempty, 0) : tempty;
+      const uint32_t my_slot = tc::smem_u32(scales + threadIdx.x);
+      constexpr int SLOT = S::groups * 128;               // floats of a depth block's rows or columns
       int it = 0; bool ok = true;
       for (int tile = first; tile < ntiles; tile += step) {
          int tp, tq; place(tile, tp, tq);
-         const int64_t p = (int64_t)tp * BM + row, q0 = (int64_t)tq * BN + col0;
-         const int64_t my_col = COLVEC ? q0 + row : q0;   // the column whose scale this thread fetches
-         const bool fetches = !COLVEC || row < CW;
-         uint64_t acc[CW / 2];
+         const int64_t p = (int64_t)tp * ROWS + prow + row, q0 = (int64_t)tq * BN + col0;
+         // Scales come AHEAD blocks early, straight to shared memory: the row's own, and one column's (of all columns
+         // where each has its own: the threads of the group fetch them for each other)
+         const int64_t my_col = COLVEC ? q0 + row : q0;
+         const bool in_p = p < a.p.rows, in_q = my_col < a.q.rows && (!COLVEC || row < CW);
+         const float *next_p = a.p.scale + (in_p ? (p >> a.p.shift) * a.p.s0 + kb0 * a.p.s1 : 0);
+         const float *next_q = a.q.scale + (in_q ? (my_col >> a.q.shift) * a.q.s0 + kb0 * a.q.s1 : 0);
+         int fetched = kb0;
+         auto fetch = [&] {
+            if (fetched < kb1) {
+               const uint32_t slot = my_slot + (fetched % AHEAD) * SLOT * 4;
+               tc::copy4(slot, next_p, in_p);
+               tc::copy4(slot + AHEAD * SLOT * 4, next_q, in_q);
+               if (in_p) next_p += a.p.s1;
+               if (in_q) next_q += a.q.s1;
+               fetched++;
+            }
+            tc::copies_commit();
+         };
 #pragma unroll
-         for (int j = 0; j < CW / 2; j++) acc[j] = 0;
-         // scales are fetched two blocks ahead
-         float sp[3], sq[3];
+         for (int d = 0; d < AHEAD - 1; d++) fetch();
+         float acc[CW];
 #pragma unroll
-         for (int d = 0; d < 2; d++) {
-            sp[d] = kb0 + d < kb1 ? scale_at(a.p, p, kb0 + d) : 0.0f;
-            sq[d] = kb0 + d < kb1 && fetches ? scale_at(a.q, my_col, kb0 + d) : 0.0f;
-         }
+         for (int j = 0; j < CW; j++) acc[j] = 0;
          for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int b = it & 1;
-            sp[2] = kb + 2 < kb1 ? scale_at(a.p, p, kb + 2) : 0.0f;
-            sq[2] = kb + 2 < kb1 && fetches ? scale_at(a.q, my_col, kb + 2) : 0.0f;
-            const float *cs = colscale + b * BN + col0;
-            if (COLVEC) {
-               if (fetches) colscale[b * BN + col0 + row] = sq[0];
+            const int b = it & 1, slot = kb % AHEAD;
+            tc::copies_wait<AHEAD - 2>();                 // this block's scales are there
+            if (COLVEC) {                                 // and the group's, and every thread is past the slot that is refilled
                if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
                else            asm volatile("bar.sync 2, 128;" ::: "memory");
             }
-            const float s0 = COLVEC ? sp[0] : sp[0] * sq[0];
-            const uint64_t s2 = tc::pair(__float_as_uint(s0), __float_as_uint(s0));
-            if (ok && !tc::bar_wait(tfull + 8 * b, (it / 2) & 1)) { ok = false; *(volatile int *)&failed = 1; }
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            fetch();
+            const float sp = scales[slot * SLOT + threadIdx.x];
+            const float *cs = scales + (AHEAD + slot) * SLOT + group * 128;
+            const float s0 = COLVEC ? sp : sp * cs[row];
+            if (ok) ok = tc::bar_wait(tfull + 8 * b, (it / 2) & 1);
+            __syncwarp();
             tc::fence_after();
-            uint32_t v[2][16];
-            tc::ld16(from + b * BN, v[0]);
+            constexpr int RUN = S::run, RUNS = CW / RUN;
+            uint32_t v[2][RUN];
+            tc::ld(from + b * BN, v[0]);
 #pragma unroll
-            for (int c = 0; c < CW / 16; c++) {
+            for (int c = 0; c < RUNS; c++) {
                tc::ld_wait(v[c & 1]);
-               if (c + 1 < CW / 16) tc::ld16(from + b * BN + 16 * (c + 1), v[(c + 1) & 1]);
-               else {
+               if (c + 1 < RUNS) tc::ld(from + b * BN + RUN * (c + 1), v[(c + 1) & 1]);
+               else {                                     // all read: the next products may overwrite it
                   tc::fence_before();
                   __syncwarp();
-                  if (lane == 0) tc::bar_arrive(tempty + 8 * b);
+                  if (lane == 0) { if (PAIR) tc::bar_arrive_at(tempty_at + 8 * b); else tc::bar_arrive(tempty + 8 * b); }
                }
 #pragma unroll
-               for (int j = 0; j < 16; j += 4) {
-                  uint64_t x = tc::pair(v[c & 1][j], v[c & 1][j + 1]), y = tc::pair(v[c & 1][j + 2], v[c & 1][j + 3]);
-                  if (COLVEC) {
-                     const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(cs + 16 * c + j);
-                     x = tc::mul2(x, w.x); y = tc::mul2(y, w.y);
+               for (int j = 0; j < RUN; j += 4) {
+                  const float4 w = COLVEC ? *reinterpret_cast<const float4 *>(cs + RUN * c + j) : make_float4(1, 1, 1, 1);
+#pragma unroll
+                  for (int k = 0; k < 4; k++) {
+                     const float x = __uint_as_float(v[c & 1][j + k]), wk = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+                     acc[RUN * c + j + k] = fmaf(COLVEC ? x * wk : x, s0, acc[RUN * c + j + k]);
                   }
-                  acc[8 * c + j / 2] = tc::fma2(x, s2, acc[8 * c + j / 2]);
-                  acc[8 * c + j / 2 + 1] = tc::fma2(y, s2, acc[8 * c + j / 2 + 1]);
                }
             }
-            sp[0] = sp[1]; sp[1] = sp[2]; sq[0] = sq[1]; sq[1] = sq[2];
          }
          if (!ok) {                                       // a wait ran out: no result is better than a wrong one
-            const uint64_t nan = 0x7FFFFFFF7FFFFFFFull;
+            failed = 1;
 #pragma unroll
-            for (int j = 0; j < CW / 2; j++) acc[j] = nan;
+            for (int j = 0; j < CW; j++) acc[j] = __int_as_float(0x7FFFFFFF);
          }
+         tc::copies_wait<0>();
+         // every thread is past the scales before the next tile's
+         if (COLVEC) { if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory"); }
          if (SPLIT) {
             // this block's part to shared memory, over the ring: all its copies have been consumed
             float *part = (float *)ring;
 #pragma unroll
-            for (int j = 0; j < CW / 2; j++) {
-               part[(col0 + 2 * j) * BM + row] = tc::lo_of(acc[j]);
-               part[(col0 + 2 * j + 1) * BM + row] = tc::hi_of(acc[j]);
-            }
-         } else if (p < a.p.rows) {
-            const int64_t es = a.half_out ? 2 : 4;
-            char *d = a.c + p * a.cp + q0 * a.cq;
-            if (a.cq == es && ((uintptr_t)d & 15) == 0) {
-               // a thread's outputs lie side by side: 16 bytes at a time
-               if (a.half_out) {
+            for (int j = 0; j < CW; j++) part[(col0 + j) * BM + row] = acc[j];
+            continue;
+         }
+         const int es = a.half_out ? 2 : 4;
+         const int64_t p0 = p - lane;
+         if (BN >= 128 && a.cq == es && (reinterpret_cast<uintptr_t>(a.c) | (uintptr_t)a.cp) % 16 == 0) {
+            if (a.half_out) store_rows<CW, true>(a, acc, out + warp * 4096, p0, q0, lane);
+            else            store_rows<CW, false>(a, acc, out + warp * 4096, p0, q0, lane);
+         } else if (p < a.p.rows) {                       // lanes side by side, or any strides
 #pragma unroll
-                  for (int j = 0; j < CW / 2; j += 4) {
-                     uint32_t w[4];
-#pragma unroll
-                     for (int k = 0; k < 4; k++) {
-                        const __half2 h = __floats2half2_rn(tc::lo_of(acc[j + k]), tc::hi_of(acc[j + k]));
-                        w[k] = *reinterpret_cast<const uint32_t *>(&h);
-                     }
-                     if (q0 + 2 * j + 8 <= a.q.rows) *reinterpret_cast<uint4 *>(d + 4 * j) = make_uint4(w[0], w[1], w[2], w[3]);
-                     else {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) if (q0 + 2 * j + k < a.q.rows) reinterpret_cast<uint16_t *>(d)[2 * j + k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
-                     }
-                  }
-               } else {
-#pragma unroll
-                  for (int j = 0; j < CW / 2; j += 2) {
-                     const float4 w = make_float4(tc::lo_of(acc[j]), tc::hi_of(acc[j]), tc::lo_of(acc[j + 1]), tc::hi_of(acc[j + 1]));
-                     if (q0 + 2 * j + 4 <= a.q.rows) *reinterpret_cast<float4 *>(d + 8 * j) = w;
-                     else {
-                        if (q0 + 2 * j < a.q.rows) reinterpret_cast<float *>(d)[2 * j] = w.x;
-                        if (q0 + 2 * j + 1 < a.q.rows) reinterpret_cast<float *>(d)[2 * j + 1] = w.y;
-                        if (q0 + 2 * j + 2 < a.q.rows) reinterpret_cast<float *>(d)[2 * j + 2] = w.z;
-                     }
-                  }
-               }
-            } else {
-#pragma unroll
-               for (int j = 0; j < CW / 2; j++) {
-                  if (q0 + 2 * j < a.q.rows) store_c(a, p, q0 + 2 * j, tc::lo_of(acc[j]));
-                  if (q0 + 2 * j + 1 < a.q.rows) store_c(a, p, q0 + 2 * j + 1, tc::hi_of(acc[j]));
-               }
-            }
+            for (int j = 0; j < CW; j++) if (q0 + j < a.q.rows) store_c(a, p, q0 + j, acc[j]);
          }
       }
    }
@@ -319,9 +371,9 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
          const int64_t p = (int64_t)tp * BM + (e & (BM - 1)), q = (int64_t)tq * BN + (e >> 7);
          if (p < a.p.rows) store_c(a, p, q, v);
       }
-      tc::cluster_sync();
    }
-   if (warp == EPI) tc::dealloc(tmem, S::tmem);
+   if (PAIR || SPLIT) tc::cluster_sync();                 // no block leaves while another reads it or signals to it
+   if (warp == EPI) tc::dealloc<PAIR>(tmem, S::tmem);
 }
 
 // ---------------------------------------------------------------------------
@@ -355,28 +407,32 @@ static int map_of(CUtensorMap *map, const Side &s, int64_t K, int box_rows)
    return 0;
 }
 
-template <int BN, bool COLVEC, bool SPLIT>
+template <int BN, bool PAIR, bool COLVEC, bool SPLIT>
 static int launch_tiles(const GemmArgs &a, int splits, int sms, cudaStream_t stream)
 {
-   using S = Shape<BN>;
+   using S = Shape<BN, PAIR>;
    CUtensorMap map_p, map_q;
-   if (map_of(&map_p, a.p, a.K, BM) != 0 || map_of(&map_q, a.q, a.K, BN) != 0) return -1;
-   auto *kernel = gemm_tiles<BN, COLVEC, SPLIT>;
+   if (map_of(&map_p, a.p, a.K, BM) != 0 || map_of(&map_q, a.q, a.K, S::rows_q) != 0) return -1;
+   auto *kernel = gemm_tiles<BN, PAIR, COLVEC, SPLIT>;
    SD_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
-   const int64_t ptiles = (a.p.rows + BM - 1) / BM, qtiles = (a.q.rows + BN - 1) / BN;
+   if (S::groups == 2) {                                  // moved registers have to be there: a block that waits for more waits for good
+      static const int registers = [&] { cudaFuncAttributes at; return cudaFuncGetAttributes(&at, kernel) == cudaSuccess ? at.numRegs : 0; }();
+      if (registers * 384 < 128 * 40 + 256 * 232) SD_ERROR("block_gemm: built with %d registers a thread, 168 are needed", registers);
+   }
+   constexpr int ROWS = PAIR ? 2 * BM : BM;
+   const int64_t ptiles = (a.p.rows + ROWS - 1) / ROWS, qtiles = (a.q.rows + BN - 1) / BN;
    const int kblocks = (int)((a.K + B8_BLOCK - 1) / B8_BLOCK);
+   const int cluster = SPLIT ? splits : PAIR ? 2 : 1;
    cudaLaunchConfig_t cfg = {};
    const int64_t room = (int64_t)sms * S::resident;
-   cfg.gridDim = dim3((unsigned)(SPLIT ? ptiles * qtiles * splits : std::min(ptiles * qtiles, room)));
+   cfg.gridDim = dim3((unsigned)(SPLIT ? ptiles * qtiles * splits : std::min(ptiles * qtiles * cluster, room / cluster * cluster)));
    cfg.blockDim = dim3(S::threads);
    cfg.dynamicSmemBytes = S::smem;
    cfg.stream = stream;
    cudaLaunchAttribute attr[1];
-   if (SPLIT) {
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = (unsigned)splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr; cfg.numAttrs = 1;
-   }
+   attr[0].id = cudaLaunchAttributeClusterDimension;
+   attr[0].val.clusterDim.x = (unsigned)cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+   if (cluster > 1) { cfg.attrs = attr; cfg.numAttrs = 1; }
    SD_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, a, splits, kblocks, (int)ptiles, (int)qtiles));
    return 0;
 }
@@ -384,8 +440,8 @@ static int launch_tiles(const GemmArgs &a, int splits, int sms, cudaStream_t str
 template <int BN> static int launch_width(const GemmArgs &a, int splits, int sms, cudaStream_t stream)
 {
    const bool vec = a.q.shift == 0;
-   if (splits > 1) return vec ? launch_tiles<BN, true, true>(a, splits, sms, stream) : launch_tiles<BN, false, true>(a, splits, sms, stream);
-   return vec ? launch_tiles<BN, true, false>(a, 1, sms, stream) : launch_tiles<BN, false, false>(a, 1, sms, stream);
+   if (splits > 1) return vec ? launch_tiles<BN, false, true, true>(a, splits, sms, stream) : launch_tiles<BN, false, false, true>(a, splits, sms, stream);
+   return vec ? launch_tiles<BN, false, true, false>(a, 1, sms, stream) : launch_tiles<BN, false, false, false>(a, 1, sms, stream);
 }
 
 static bool on_boundaries(const Side &s, int64_t K)
@@ -426,7 +482,8 @@ static int gemm(GemmArgs &a, cudaStream_t stream)
       case 32:  return launch_width<32>(a, splits, dev.sms, stream);
       case 64:  return launch_width<64>(a, splits, dev.sms, stream);
       case 128: return launch_width<128>(a, splits, dev.sms, stream);
-      default:  return launch_width<256>(a, splits, dev.sms, stream);
+      default:  return a.q.shift == 0 ? launch_tiles<256, true, true, false>(a, 1, dev.sms, stream)
+                                      : launch_tiles<256, true, false, false>(a, 1, dev.sms, stream);
    }
 }
 

@@ -36,12 +36,31 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity)
       if (clock64() - from > WAIT_CYCLES) return false;
    return true;
 }
-
-// A box of a two-dimensional tensor to shared memory
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
+// The address of the same place in block `rank` of the cluster
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank)
 {
-   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+   uint32_t there;
+   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+   return there;
+}
+// An arrival at another block's barrier.  It orders tensor memory (with tcgen05.fence around it), not shared or global
+// memory, so it goes without a release for the cluster, which costs about 1000 cycles.
+__device__ __forceinline__ void bar_arrive_at(uint32_t cluster_addr)
+{
+   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
+}
+
+// PAIR: two blocks of a cluster work on one tile of twice the rows; block 0 issues the products for both.
+
+// A box of a two-dimensional tensor to this block's shared memory; in a pair the barrier may be block 0's
+template <bool PAIR> __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
+{
+   if (PAIR)
+      asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                   :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+   else
+      asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                   :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 
 // Rows of 128 bytes, side by side in groups of eight (1024 bytes), 128-byte swizzle, contiguous along the depth
@@ -51,50 +70,83 @@ __device__ __forceinline__ uint64_t tile_descriptor(uint32_t addr)
 }
 
 // D (+)= A B, 8-bit floating-point operands from shared memory, 32-bit sums in tensor memory, depth 32
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+template <bool PAIR> __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
 {
-   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-                "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
-                :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+   if (PAIR)
+      asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                   "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                   :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+   else
+      asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                   "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                   :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t bar)
+// Arrives on the barrier (of both blocks of a pair) when the products issued so far are done
+template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar)
 {
-   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+   if (PAIR)
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                   :: "r"(bar), "h"((uint16_t)3) : "memory");
+   else
+      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after()  { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void alloc(uint32_t where, uint32_t columns)
+template <bool PAIR> __device__ __forceinline__ void alloc(uint32_t where, uint32_t columns)
 {
-   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(where), "r"(columns) : "memory");
-   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+   if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(where), "r"(columns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+   } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(where), "r"(columns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+   }
 }
-__device__ __forceinline__ void dealloc(uint32_t addr, uint32_t columns)
+template <bool PAIR> __device__ __forceinline__ void dealloc(uint32_t addr, uint32_t columns)
 {
-   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
+   if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
+   else      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
 }
 
-// Sixteen columns of a warp's 32 lanes; the values may be used after ld_wait on the same registers
-__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&v)[16])
+// 8, 16 or 32 columns of a warp's 32 lanes; the values may be used after ld_wait on the same registers
+__device__ __forceinline__ void ld(uint32_t addr, uint32_t (&v)[8])
+{
+   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                : "r"(addr));
+}
+__device__ __forceinline__ void ld_wait(uint32_t (&v)[8])
+{
+   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]));
+}
+__device__ __forceinline__ void ld(uint32_t addr, uint32_t (&v)[16])
 {
    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                  "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                 : "r"(addr));
 }
 __device__ __forceinline__ void ld_wait(uint32_t (&v)[16])
 {
-   asm volatile("tcgen05.wait::ld.sync.aligned;"
-                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                  "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]));
+   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]));
+}
+__device__ __forceinline__ void ld(uint32_t addr, uint32_t (&v)[32])
+{
+   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                  "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+                  "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                : "r"(addr));
+}
+__device__ __forceinline__ void ld_wait(uint32_t (&v)[32])
+{
+   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
 
-// Two 32-bit operations in one instruction
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi)); return r; }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+// A warpgroup's registers a thread
+template <int N> __device__ __forceinline__ void registers_up()   { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
 
 __device__ __forceinline__ void cluster_sync()
 {
@@ -103,10 +155,17 @@ __device__ __forceinline__ void cluster_sync()
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ float peer_load(uint32_t addr, uint32_t rank)
 {
-   uint32_t there; float v;
-   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+   float v;
+   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at_rank(addr, rank)) : "memory");
    return v;
 }
+
+// Four bytes to shared memory without a register in between; `in` false: zero
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool in)
+{
+   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
 } } // namespace sd::tc
