@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(256) gemm_plain(const __grid_constant__ GemmAr
 constexpr int BM = 128;
 constexpr int TILE_P = BM * B8_BLOCK;                     // bytes of a stage's 128 rows
 
-constexpr int AHEAD = 4;                                  // depth blocks whose scales are under way
+constexpr int AHEAD = 8;                                  // places for depth blocks' scales
 
 // PAIR: two blocks share a tile of 256 rows, each holds half of either operand's rows; the columns' half travels once
 // instead of twice, and the 64 bytes a cycle that a block can take in no longer bound the products.
@@ -291,26 +291,36 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
          };
 #pragma unroll
          for (int d = 0; d < AHEAD - 1; d++) fetch();
-         float acc[CW];
+         uint64_t sum[CW / 2];                            // pairs of neighbouring columns
 #pragma unroll
-         for (int j = 0; j < CW; j++) acc[j] = 0;
-         for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int b = it & 1, slot = kb % AHEAD;
-            tc::copies_wait<AHEAD - 2>();                 // this block's scales are there
-            if (COLVEC) {                                 // and the group's, and every thread is past the slot that is refilled
-               if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-               else            asm volatile("bar.sync 2, 128;" ::: "memory");
-            }
-            fetch();
+         for (int j = 0; j < CW / 2; j++) sum[j] = 0;
+         // Everything that the next block needs is under way before the present block's sums are done: its scales are
+         // read, its first columns are on their way from tensor memory.
+         auto scale_of = [&](int kb) {
+            const int slot = kb % AHEAD;
             const float sp = scales[slot * SLOT + threadIdx.x];
-            const float *cs = scales + (AHEAD + slot) * SLOT + group * 128;
-            const float s0 = COLVEC ? sp : sp * cs[row];
-            if (ok) ok = tc::bar_wait(tfull + 8 * b, (it / 2) & 1);
+            return COLVEC ? sp : sp * scales[(AHEAD + slot) * SLOT + threadIdx.x];
+         };
+         auto group_sync = [&] {
+            if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+            else            asm volatile("bar.sync 2, 128;" ::: "memory");
+         };
+         auto wait_sums = [&](int i) {
+            if (ok) ok = tc::bar_wait(tfull + 8 * (i & 1), (i / 2) & 1);
             __syncwarp();
             tc::fence_after();
-            constexpr int RUN = S::run, RUNS = CW / RUN;
-            uint32_t v[2][RUN];
-            tc::ld(from + b * BN, v[0]);
+         };
+         constexpr int RUN = S::run, RUNS = CW / RUN;     // an even number: a block's first run is in v[0]
+         uint32_t v[2][RUN];
+         tc::copies_wait<AHEAD - 2>();
+         if (COLVEC) group_sync();
+         float s = scale_of(kb0);
+         wait_sums(it);
+         tc::ld(from + (it & 1) * BN, v[0]);
+         for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int b = it & 1;
+            const float *cs = scales + (AHEAD + kb % AHEAD) * SLOT + group * 128;
+            const uint64_t s2 = tc::pair(__float_as_uint(s), __float_as_uint(s));
 #pragma unroll
             for (int c = 0; c < RUNS; c++) {
                tc::ld_wait(v[c & 1]);
@@ -319,26 +329,37 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
                   tc::fence_before();
                   __syncwarp();
                   if (lane == 0) { if (PAIR) tc::bar_arrive_at(tempty_at + 8 * b); else tc::bar_arrive(tempty + 8 * b); }
+                  if (kb + 1 < kb1) { wait_sums(it + 1); tc::ld(from + (b ^ 1) * BN, v[0]); }
+               }
+               if (c == 0) {
+                  tc::copies_wait<AHEAD - 3>();           // the next block's scales, of every thread of the group
+                  if (COLVEC) group_sync();               // which is also past the place that is filled again
+                  fetch();
+                  s = scale_of(kb + 1 < kb1 ? kb + 1 : kb);
                }
 #pragma unroll
                for (int j = 0; j < RUN; j += 4) {
-                  const float4 w = COLVEC ? *reinterpret_cast<const float4 *>(cs + RUN * c + j) : make_float4(1, 1, 1, 1);
-#pragma unroll
-                  for (int k = 0; k < 4; k++) {
-                     const float x = __uint_as_float(v[c & 1][j + k]), wk = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
-                     acc[RUN * c + j + k] = fmaf(COLVEC ? x * wk : x, s0, acc[RUN * c + j + k]);
+                  uint64_t x = tc::pair(v[c & 1][j], v[c & 1][j + 1]), y = tc::pair(v[c & 1][j + 2], v[c & 1][j + 3]);
+                  if (COLVEC) {
+                     const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(cs + RUN * c + j);
+                     x = tc::mul2(x, w.x); y = tc::mul2(y, w.y);
                   }
+                  const int k = (RUN * c + j) / 2;
+                  sum[k] = tc::fma2(x, s2, sum[k]);
+                  sum[k + 1] = tc::fma2(y, s2, sum[k + 1]);
                }
             }
          }
+         float acc[CW];
+#pragma unroll
+         for (int j = 0; j < CW / 2; j++) { acc[2 * j] = tc::lo_of(sum[j]); acc[2 * j + 1] = tc::hi_of(sum[j]); }
          if (!ok) {                                       // a wait ran out: no result is better than a wrong one
             failed = 1;
 #pragma unroll
             for (int j = 0; j < CW; j++) acc[j] = __int_as_float(0x7FFFFFFF);
          }
          tc::copies_wait<0>();
-         // every thread is past the scales before the next tile's
-         if (COLVEC) { if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory"); }
+         if (COLVEC) group_sync();                        // every thread is past the scales before the next tile's
          if (SPLIT) {
             // this block's part to shared memory, over the ring: all its copies have been consumed
             float *part = (float *)ring;
