@@ -186,7 +186,7 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
    char *out = ring + ST * S::stage + S::scales;
    const uint32_t ring_u = tc::smem_u32(ring);
    const uint32_t full = tc::smem_u32(bars), empty = full + 8 * ST, tfull = full + 16 * ST, tempty = tfull + 16;
-   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
    constexpr int EPI = S::groups * 4;                     // epilogue warps come first: warp w reads lanes 32 (w % 4)
    const int rank = PAIR || SPLIT ? (int)tc::cluster_rank() : 0;
    const bool leader = !PAIR || rank == 0;
@@ -222,38 +222,45 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
 
    if (warp >= EPI) {
       if (S::groups == 2) tc::registers_down<40>();
-      if (warp == EPI && lane == 0) {                     // ---- loads
+      // s and turn: place in the ring, and how often it came round; b and round the same for tensor memory
+      if (warp == EPI) {                                  // ---- loads
          const uint32_t full_at = PAIR ? tc::at_rank(full, 0) : full;
-         int it = 0; bool ok = true;
+         int it = 0, s = 0; uint32_t turn = 0; bool ok = true;
          for (int tile = first; tile < ntiles && ok; tile += step) {
             int tp, tq; place(tile, tp, tq);
             for (int kb = kb0; kb < kb1; kb++, it++) {
-               const int s = it % ST;
-               if (it >= ST && !tc::bar_wait(empty + 8 * s, (it / ST - 1) & 1)) { ok = false; break; }
-               const uint32_t dst = ring_u + s * S::stage;
-               if (leader) tc::bar_expect(full + 8 * s, PAIR ? 2 * S::stage : S::stage);
-               tc::load_box<PAIR>(dst, &map_p, full_at + 8 * s, kb * B8_BLOCK, tp * ROWS + prow);
-               tc::load_box<PAIR>(dst + TILE_P, &map_q, full_at + 8 * s, kb * B8_BLOCK, tq * BN + qrow);
+               if (it >= ST && !tc::bar_wait_warp(empty + 8 * s, turn ^ 1)) { ok = false; break; }
+               if (tc::elect()) {
+                  const uint32_t dst = ring_u + s * S::stage;
+                  if (leader) tc::bar_expect(full + 8 * s, PAIR ? 2 * S::stage : S::stage);
+                  tc::load_box<PAIR>(dst, &map_p, full_at + 8 * s, kb * B8_BLOCK, tp * ROWS + prow);
+                  tc::load_box<PAIR>(dst + TILE_P, &map_q, full_at + 8 * s, kb * B8_BLOCK, tq * BN + qrow);
+               }
+               if (++s == ST) { s = 0; turn ^= 1; }
             }
          }
          if (!ok) {                                       // the copies under way end before shared memory is given back
             *(volatile int *)&failed = 1;
             if (leader) for (int k = max(0, it - ST); k < it; k++) tc::bar_wait(full + 8 * (k % ST), (k / ST) & 1);
          }
-      } else if (warp == EPI + 1 && lane == 0 && leader) {   // ---- products
+      } else if (warp == EPI + 1 && leader) {             // ---- products
          const uint32_t idesc = (1u << 4) | ((uint32_t)a.p.format << 7) | ((uint32_t)a.q.format << 10) | ((uint32_t)(BN / 8) << 17) | ((uint32_t)(ROWS / 16) << 24);
-         int it = 0; bool ok = true;
+         const uint64_t desc_p = tc::tile_descriptor(ring_u), desc_q = tc::tile_descriptor(ring_u + TILE_P);
+         int it = 0, s = 0; uint32_t turn = 0, b = 0, round = 0; bool ok = true;
          for (int tile = first; tile < ntiles && ok; tile += step)
             for (int kb = kb0; kb < kb1; kb++, it++) {
-               const int s = it % ST, b = it & 1;
-               if (it >= 2 && !tc::bar_wait(tempty + 8 * b, (it / 2 - 1) & 1)) { ok = false; break; }
-               if (!tc::bar_wait(full + 8 * s, (it / ST) & 1)) { ok = false; break; }
+               if (it >= 2 && !tc::bar_wait_warp(tempty + 8 * b, round ^ 1)) { ok = false; break; }
+               if (!tc::bar_wait_warp(full + 8 * s, turn)) { ok = false; break; }
                tc::fence_after();
-               const uint64_t dp = tc::tile_descriptor(ring_u + s * S::stage), dq = tc::tile_descriptor(ring_u + s * S::stage + TILE_P);
+               if (tc::elect()) {
+                  const uint64_t dp = desc_p + (uint32_t)(s * S::stage / 16), dq = desc_q + (uint32_t)(s * S::stage / 16);
 #pragma unroll
-               for (int k = 0; k < 4; k++) tc::mma_f8<PAIR>(tmem + b * BN, dp + 2 * k, dq + 2 * k, idesc, k > 0);
-               tc::commit<PAIR>(empty + 8 * s);
-               tc::commit<PAIR>(tfull + 8 * b);
+                  for (int k = 0; k < 4; k++) tc::mma_f8<PAIR>(tmem + b * BN, dp + 2 * k, dq + 2 * k, idesc, k > 0);
+                  tc::commit<PAIR>(empty + 8 * s);
+                  tc::commit<PAIR>(tfull + 8 * b);
+               }
+               if (++s == ST) { s = 0; turn ^= 1; }
+               b ^= 1; if (b == 0) round ^= 1;
             }
          if (!ok) {
             *(volatile int *)&failed = 1;

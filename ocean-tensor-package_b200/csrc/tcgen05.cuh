@@ -36,6 +36,16 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity)
       if (clock64() - from > WAIT_CYCLES) return false;
    return true;
 }
+// For a warp that waits as one
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity)); }
+// One lane of a whole warp.  The loops that issue copies and products are run by all lanes, so that addresses and
+// descriptors stay in uniform registers, and only the instructions themselves by one.
+__device__ __forceinline__ bool elect()
+{
+   uint32_t yes;
+   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+   return yes != 0;
+}
 // The address of the same place in block `rank` of the cluster
 __device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank)
 {
