@@ -1,6 +1,6 @@
 // solid_gpu_block_quantize: the codes and scales of a matrix, a scale for 128 elements of dimension 0 by 1 or 128 rows.
 //
-// Bound by memory: a block of 256 threads loads a 128 x 128 tile once into registers, finds the largest magnitudes,
+// Bound by memory: a block of 256 threads loads a tile (128 x 64, 128 x 128) once into registers, finds the largest magnitudes,
 // and writes the codes.  The tile is read along whichever dimension of the source is contiguous, eight elements a
 // thread; where that is the rows' dimension (the codes of a transposed matrix) the codes turn in shared memory, one
 // byte each, so that both sides of the copy move whole lines.
@@ -16,37 +16,46 @@ struct QuantArgs {
    int format;
 };
 
-constexpr int QT = 128;                                   // tile edge
+constexpr int QT = 128;                                   // tile edge along dimension 0
 
-// Values of one thread: eight runs of eight.  Doubles are taken in 32 bits, as the scales are.
+// Values of one thread: runs of eight.  Doubles are taken in 32 bits, as the scales are.
 template <class T> struct Held { using type = T; };
 template <> struct Held<double> { using type = float; };
 
+// RB: rows that share a scale.  Where each row has its own a tile takes 64 rows, so that more and smaller blocks are on an
+// SM and one's loads run beside another's stores; 128 by 128 it has to be for a common scale.
+template <class T, int RB> struct QuantShape {
+   static constexpr int rows = RB == 1 ? 64 : QT;
+   static constexpr int runs = rows / 16;                 // of a thread
+   static constexpr int resident = RB == 1 ? (sizeof(T) == 2 ? 5 : 4) : sizeof(T) == 2 ? 3 : 2;
+};
+
 // ACROSS: the source is contiguous along the rows' dimension.  VEC: runs of eight start on 16-byte boundaries.
-// RB: rows that share a scale.
 template <class T, bool ACROSS, bool VEC, int RB>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tiles(const __grid_constant__ QuantArgs a)
+__global__ void __launch_bounds__(256, QuantShape<T, RB>::resident) quantize_tiles(const __grid_constant__ QuantArgs a)
 {
    using H = typename Held<T>::type;
+   constexpr int QR = QuantShape<T, RB>::rows, P = QuantShape<T, RB>::runs;
+   constexpr int TX = ACROSS ? QR / 8 : QT / 8;           // threads side by side along the contiguous dimension
    __shared__ uint32_t most[QT];
    __shared__ alignas(16) float inverse[QT];
-   __shared__ alignas(16) unsigned char turned[ACROSS ? QT * QT : 16];
-   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, lane = threadIdx.x & 31;
-   const int64_t ntiles = (a.n + QT - 1) / QT, rtiles = (a.rows + QT - 1) / QT;
+   __shared__ alignas(16) unsigned char turned[ACROSS ? QR * QT : 16];
+   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, lane = threadIdx.x & 31;
+   const int64_t ntiles = (a.n + QT - 1) / QT, rtiles = (a.rows + QR - 1) / QR;
    // neighbouring blocks take neighbouring tiles of the contiguous dimension
    const int64_t tile_n = ACROSS ? blockIdx.x / rtiles : blockIdx.x % ntiles;
    const int64_t tile_r = ACROSS ? blockIdx.x % rtiles : blockIdx.x / ntiles;
-   const int64_t i0 = tile_n * QT, r0 = tile_r * QT;
+   const int64_t i0 = tile_n * QT, r0 = tile_r * QR;
    // run p of a thread lies at `other(p)` of the dimension that is not contiguous; element j of it at `along(j)` of the
    // contiguous one.  Scalar accesses interleave the lanes.
-   auto along = [&](int j) { return VEC ? tx * 8 + j : tx + 16 * j; };
-   auto other = [&](int p) { return ACROSS ? ty * 8 + p : p * 16 + ty; };
+   auto along = [&](int j) { return VEC ? tx * 8 + j : tx + TX * j; };
+   auto other = [&](int p) { return ACROSS ? ty * P + p : p * 16 + ty; };
    const int64_t along_left = ACROSS ? a.rows - r0 : a.n - i0, other_left = ACROSS ? a.n - i0 : a.rows - r0;
    const int64_t along_step = ACROSS ? a.s1 : a.s0, other_step = ACROSS ? a.s0 : a.s1;
    const char *base = a.x + i0 * a.s0 + r0 * a.s1;
-   H v[8][8];
+   H v[P][8];
 #pragma unroll
-   for (int p = 0; p < 8; p++) {
+   for (int p = 0; p < P; p++) {
       const char *q = base + other(p) * other_step;
       const bool in = other(p) < other_left;
       if (VEC && in && tx * 8 + 8 <= along_left) {
@@ -61,7 +70,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tiles(co
    auto value = [&](int p, int j) { return to_acc(v[p][j]); };
    auto store_scale = [&](int64_t row_block, float s) { a.scale[row_block * a.ss0 + tile_n * a.ss1] = s; };
 
-   float scale_one = 0, inv_one = 0, inv[8];
+   float inv[8];                                          // of the thread's runs, ACROSS of its elements
    if (RB == QT || ACROSS) {                              // maxima meet in shared memory
       if (threadIdx.x < QT) most[threadIdx.x] = 0;
       __syncthreads();
@@ -69,29 +78,28 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tiles(co
    if (RB == QT) {
       uint32_t m = 0;
 #pragma unroll
-      for (int p = 0; p < 8; p++)
+      for (int p = 0; p < P; p++)
 #pragma unroll
          for (int j = 0; j < 8; j++) m = max(m, b8_magnitude(value(p, j)));
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+      m = __reduce_max_sync(0xFFFFFFFFu, m);
       if (lane == 0) atomicMax(&most[0], m);              // a maximum of whole numbers: any order gives the same
       __syncthreads();
-      scale_one = b8_scale(most[0], a.format);
-      inv_one = 1.0f / scale_one;
-      if (threadIdx.x == 0) store_scale(tile_r, scale_one);
+      const float s = b8_scale(most[0], a.format);
+      if (threadIdx.x == 0) store_scale(tile_r, s);
 #pragma unroll
-      for (int k = 0; k < 8; k++) inv[k] = inv_one;
-   } else if (ACROSS) {                                   // a row is one j of 16 threads
+      for (int k = 0; k < 8; k++) inv[k] = 1.0f / s;
+   } else if (ACROSS) {                                   // a row is one j of 256 / TX threads
 #pragma unroll
       for (int j = 0; j < 8; j++) {
          uint32_t m = 0;
 #pragma unroll
-         for (int p = 0; p < 8; p++) m = max(m, b8_magnitude(value(p, j)));
-         m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-         if (lane < 16) atomicMax(&most[along(j)], m);
+         for (int p = 0; p < P; p++) m = max(m, b8_magnitude(value(p, j)));
+#pragma unroll
+         for (int d = 16; d >= TX; d >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+         if (lane < TX) atomicMax(&most[along(j)], m);
       }
       __syncthreads();
-      if (threadIdx.x < QT) {
+      if (threadIdx.x < QR) {
          const float s = b8_scale(most[threadIdx.x], a.format);
          inverse[threadIdx.x] = 1.0f / s;
          if (threadIdx.x < along_left) store_scale(r0 + threadIdx.x, s);
@@ -101,7 +109,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tiles(co
       for (int j = 0; j < 8; j++) inv[j] = inverse[along(j)];
    } else {                                               // a row is one p of 16 lanes
 #pragma unroll
-      for (int p = 0; p < 8; p++) {
+      for (int p = 0; p < P; p++) {
          uint32_t m = 0;
 #pragma unroll
          for (int j = 0; j < 8; j++) m = max(m, b8_magnitude(value(p, j)));
@@ -116,7 +124,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tiles(co
    if (!ACROSS) {
       const bool whole_out = VEC && (reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.ld) % 8 == 0;
 #pragma unroll
-      for (int p = 0; p < 8; p++) {
+      for (int p = 0; p < P; p++) {
          if (other(p) >= other_left) continue;
          char *q = a.codes + i0 + (r0 + other(p)) * a.ld;
          float f[8];
@@ -130,30 +138,37 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tiles(co
          }
       }
    } else {
-      // Row `along(j)` gets the eight codes of this thread at element ty * 8, one of the row's sixteen 8-byte places.
-      // Places are permuted by the row, so that the sixteen lanes with one ty write to different banks.
-      auto place = [](int row, int k) { return row * QT + ((k ^ (VEC ? row >> 3 : row & 15)) * 8); };
+      // Row `along(j)` gets this thread's P codes at element ty * P.  A row's places of P bytes are permuted by the row,
+      // so that the lanes of a warp write to different banks; 16 bytes stay together in steps of P.
+      auto turn = [](int row) { return VEC ? row >> 3 : row % TX; };
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-         float f[8];
+         float f[P];
 #pragma unroll
-         for (int p = 0; p < 8; p++) f[p] = value(p, j);
-         *reinterpret_cast<uint2 *>(turned + place(along(j), ty)) = make_uint2(b8_four(f, inv[j], a.format), b8_four(f + 4, inv[j], a.format));
+         for (int p = 0; p < P; p++) f[p] = value(p, j);
+         const int row = along(j);
+         unsigned char *d = turned + row * QT + (P == 8 ? (ty ^ turn(row)) * 8 : (ty ^ (turn(row) * 4)) * 4);
+         if constexpr (P == 8) *reinterpret_cast<uint2 *>(d) = make_uint2(b8_four(f, inv[j], a.format), b8_four(f + 4, inv[j], a.format));
+         else *reinterpret_cast<uint32_t *>(d) = b8_four(f, inv[j], a.format);
       }
       __syncthreads();
       const bool whole_out = (reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.ld) % 16 == 0;
       const int part = threadIdx.x & 7;
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
+      for (int q = 0; q < QR / 32; q++) {
          const int row = (threadIdx.x >> 3) + 32 * q;
          if (row >= along_left) continue;
-         const uint2 lo = *reinterpret_cast<const uint2 *>(turned + place(row, 2 * part));
-         const uint2 hi = *reinterpret_cast<const uint2 *>(turned + place(row, 2 * part + 1));
+         uint4 w;
+         if constexpr (P == 8) {
+            const uint2 lo = *reinterpret_cast<const uint2 *>(turned + row * QT + ((2 * part) ^ turn(row)) * 8);
+            const uint2 hi = *reinterpret_cast<const uint2 *>(turned + row * QT + ((2 * part + 1) ^ turn(row)) * 8);
+            w = make_uint4(lo.x, lo.y, hi.x, hi.y);
+         } else w = *reinterpret_cast<const uint4 *>(turned + row * QT + (part ^ turn(row)) * 16);
          const int64_t left = other_left - part * 16;
          char *d = a.codes + i0 + part * 16 + (r0 + row) * a.ld;
-         if (whole_out && left >= 16) *reinterpret_cast<uint4 *>(d) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+         if (whole_out && left >= 16) *reinterpret_cast<uint4 *>(d) = w;
          else {
-            const uint32_t word[4] = { lo.x, lo.y, hi.x, hi.y };
+            const uint32_t word[4] = { w.x, w.y, w.z, w.w };
 #pragma unroll
             for (int k = 0; k < 16; k++) if (k < left) d[k] = (char)(word[k >> 2] >> (8 * (k & 3)));
          }
@@ -171,7 +186,8 @@ static void quantize_launch(const QuantArgs &a, int block, unsigned int grid, cu
 template <class T> static int quantize_typed(const QuantArgs &a, int block, cudaStream_t stream)
 {
    const int64_t es = (int64_t)sizeof(T);
-   const int64_t ntiles = (a.n + QT - 1) / QT, rtiles = (a.rows + QT - 1) / QT, tiles = ntiles * rtiles;
+   const int64_t edge = block == 1 ? QuantShape<T, 1>::rows : QT;
+   const int64_t ntiles = (a.n + QT - 1) / QT, rtiles = (a.rows + edge - 1) / edge, tiles = ntiles * rtiles;
    if (ntiles > 0x7FFFFFFF / rtiles) SD_ERROR("block_quantize: matrix too large");
    auto magnitude = [](int64_t v) { return v < 0 ? -v : v; };
    const bool across = magnitude(a.s1) < magnitude(a.s0) && a.rows > 1;

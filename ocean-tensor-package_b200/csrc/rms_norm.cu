@@ -555,23 +555,26 @@ __global__ void __launch_bounds__(MAXT) grad_ring(const __grid_constant__ GradAr
    }
 }
 
-// dw = the sum of the blocks' partial rows, in the order of the blocks
+// dw = the sum of the blocks' partial rows: 32 columns a block, its warps a part of the rows each, in the order of the
+// blocks within a warp and then of the warps
+constexpr int JOIN_WARPS = 32;
 template <class W>
-__global__ void __launch_bounds__(256) grad_join(const W *__restrict__ part, int64_t parts, int64_t n, W *__restrict__ dw)
+__global__ void __launch_bounds__(JOIN_WARPS * 32) grad_join(const W *__restrict__ part, int64_t parts, int64_t n, W *__restrict__ dw)
 {
-   __shared__ W sums[8][33];
+   __shared__ W sums[JOIN_WARPS][33];
    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
    const int64_t k = (int64_t)blockIdx.x * 32 + lane;
    W s = 0;
    if (k < n)
 #pragma unroll 8
-      for (int64_t p = warp; p < parts; p += 8) s += part[p * n + k];
+      for (int64_t p = warp; p < parts; p += JOIN_WARPS) s += part[p * n + k];
    sums[warp][lane] = s;
    __syncthreads();
-   if (warp == 0 && k < n) {
-      for (int q = 1; q < 8; q++) s += sums[q][lane];
-      dw[k] = s;
-   }
+   s = sums[lane][warp];                                  // column `warp` of the block's, a part each lane
+#pragma unroll
+   for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+   const int64_t c = (int64_t)blockIdx.x * 32 + warp;
+   if (lane == 0 && c < n) dw[c] = s;
 }
 
 // Long rows: a first kernel forms each row's r and r^3 mean(g h), a second one walks the columns
@@ -803,7 +806,7 @@ static GradPlan grad_plan(int64_t n, int64_t rows, size_t elemsize, int sms)
    else if (n <= NORM_MAX && !wide) { p.kind = 14; p.threads = round32((eights + 3) / 4); }
    else                { p.kind = 20; p.threads = 256; }
    const int64_t rows_at_once = p.kind < 10 ? 8 : 1;      // warps of a block
-   const int64_t most = p.kind == 20 ? 16 : (int64_t)sms * std::min(4, std::max(1, 512 / p.threads));
+   const int64_t most = p.kind == 20 ? 16 : (int64_t)sms * std::min(2, std::max(1, 512 / p.threads));
    const int64_t want = (rows + rows_at_once - 1) / rows_at_once;
    p.blocks = (int)std::max<int64_t>(1, std::min(want, most));
    return p;
@@ -867,7 +870,7 @@ template <class T> static int grad_typed(GradArgs &a, void *dw, void *buffer, cu
    else if ((grad_vec<T>(a) ? grad_of<T, true>(a, p, dev.sms, stream) : grad_of<T, false>(a, p, dev.sms, stream)) != 0) return -1;
    SD_LAUNCH_CHECK();
    if (dw != nullptr) {
-      grad_join<W><<<(unsigned)((a.n + 31) / 32), 256, 0, stream>>>(part, p.blocks, a.n, (W *)dw);
+      grad_join<W><<<(unsigned)((a.n + 31) / 32), JOIN_WARPS * 32, 0, stream>>>(part, p.blocks, a.n, (W *)dw);
       SD_LAUNCH_CHECK();
    }
    return 0;
