@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(512) norm_long(const __grid_constant__ NormArg
 // gradient
 // ---------------------------------------------------------------------------
 template <class T, int V, bool BLOCK, bool VEC, bool PIPE, int MAXT>
-__global__ void __launch_bounds__(MAXT) grad_rows(const __grid_constant__ GradArgs a)
+__global__ void __launch_bounds__(MAXT, BLOCK || sizeof(T) == 8 ? 1 : 3) grad_rows(const __grid_constant__ GradArgs a)
 {
    using W = typename Real<T>::acc;
    __shared__ W sums[2][2][32];
@@ -690,16 +690,21 @@ static int launch_norm(NormArgs &a, int threads, int sms, cudaStream_t stream)
    return 0;
 }
 
-// Shared memory of an SM, shared by as many blocks as keep 1024 threads or so on it
+// Blocks of an SM and rows under way in each.  About 128 KB under way on an SM are enough for the memory's latency, more
+// only disturbs (halves, n 4096 with residual: 45 us with 128 KB, 49 us with 190 KB); four rows a block spread over
+// enough blocks for the arithmetic, which with 8-bit output is twice as much (n 4096: 58 us with 512 threads an SM, 47 us
+// with 1024).
 struct RingPlan { int per_sm, stages; size_t smem; };
-static RingPlan ring_plan(int64_t stage_bytes, int threads)
+static RingPlan ring_plan(int64_t stage_bytes, int threads, int threads_per_sm)
 {
+   constexpr int64_t UNDER_WAY = 128 * 1024, ROOM = 225 * 1024;
    RingPlan p;
-   for (p.per_sm = std::min(4, std::max(1, 1024 / threads)); p.per_sm >= 1; p.per_sm--) {
-      p.stages = (int)std::min<int64_t>(RING_MAX, (225 * 1024 / p.per_sm - 2048) / stage_bytes);
-      if (p.stages >= 3 || (p.per_sm == 1 && p.stages == 2)) break;
-   }
-   p.smem = p.per_sm >= 1 ? (size_t)(p.stages * stage_bytes) : 0;
+   p.per_sm = (int)std::min<int64_t>(16, std::max<int64_t>(UNDER_WAY / (RING_MAX * stage_bytes), threads_per_sm / threads));
+   p.per_sm = std::max(1, std::min(p.per_sm, 2048 / threads));
+   while (p.per_sm > 1 && 2 * stage_bytes > ROOM / p.per_sm - 2048) p.per_sm--;
+   p.stages = (int)std::max<int64_t>(2, std::min<int64_t>(RING_MAX, (p.per_sm > 1 ? UNDER_WAY : ROOM - 2048) / (p.per_sm * stage_bytes)));
+   p.smem = (size_t)(p.stages * stage_bytes);
+   if (2 * stage_bytes > ROOM - 2048) p.per_sm = 0;       // not even two rows: no ring
    return p;
 }
 
@@ -729,12 +734,11 @@ static int norm_of(NormArgs &a, cudaStream_t stream)
    if constexpr (VEC) {
       if (n <= NORM_MAX) {
          const int threads = std::max(64, round32((eights + (n <= 8192 ? 1 : 3)) / (n <= 8192 ? 2 : 4)));
-         const RingPlan p = ring_plan(n * (int64_t)sizeof(T) * (a.res.p != nullptr ? 2 : 1), threads);
+         const RingPlan p = ring_plan(n * (int64_t)sizeof(T) * (a.res.p != nullptr ? 2 : 1), threads, QUANT ? 1024 : 512);
          if (p.per_sm >= 1) return n <= 8192 ? launch_norm_ring<T, 2, QUANT>(a, p, threads, sms, stream)
                                              : launch_norm_ring<T, 4, QUANT>(a, p, threads, sms, stream);
       }
    }
-   if (n <= 1024) return launch_norm<T, 4, false, VEC, !WIDE, QUANT, 256>(a, 256, sms, stream);
    if (n <= 2048) return launch_norm<T, 1, true, VEC, true, QUANT, 256>(a, round32(eights), sms, stream);
    if (n <= 8192) return launch_norm<T, 2, true, VEC, !WIDE, QUANT, 512>(a, round32((eights + 1) / 2), sms, stream);
    if constexpr (!WIDE) {
@@ -783,8 +787,13 @@ static int fill_norm(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x
 }
 
 // ---- gradient ----
-// kind: 1, 2 eights of a warp's thread; 11, 12, 14 of a block's; 20 long rows
+// kind: 1 a warp's row; 11, 12, 14 a block's, with 1, 2, 4 eights a thread; 20 long rows
 struct GradPlan { int kind, threads, blocks; };
+
+static int grad_stages(int64_t n, size_t elemsize, int operands, int per_sm)
+{
+   return (int)std::min<int64_t>(RING_MAX, (225 * 1024 / per_sm - 2048) / (n * (int64_t)elemsize * operands));
+}
 
 template <class T> static bool grad_vec(const GradArgs &a)
 {
@@ -794,21 +803,24 @@ template <class T> static bool grad_vec(const GradArgs &a)
 }
 
 // The number of partial rows follows from sizes alone, so that the buffer's size can be asked for beforehand and the
-// order of the sums does not depend on addresses.
+// order of the sums does not depend on addresses.  Blocks of an SM: 1024 threads, as long as three operands' rows fit
+// the ring twice (halves, n 4096: 34 us with 512 threads, 30 us with 1024).
 static GradPlan grad_plan(int64_t n, int64_t rows, size_t elemsize, int sms)
 {
    const bool wide = elemsize == 8;
    const int64_t eights = (n + 7) / 8;
    GradPlan p;
-   if (n <= 512)       { p.kind = n <= 256 ? 1 : 2; p.threads = 256; }
+   if (n <= 256)       { p.kind = 1; p.threads = 256; }
    else if (n <= 1024) { p.kind = 11; p.threads = round32(eights); }
    else if (n <= 8192) { p.kind = 12; p.threads = round32((eights + 1) / 2); }
    else if (n <= NORM_MAX && !wide) { p.kind = 14; p.threads = round32((eights + 3) / 4); }
    else                { p.kind = 20; p.threads = 256; }
+   int per_sm = std::max(1, std::min(16, 1024 / p.threads));
+   if (p.kind == 1) per_sm = 3;
+   else while (per_sm > 1 && grad_stages(n, elemsize, 3, per_sm) < 2) per_sm--;
    const int64_t rows_at_once = p.kind < 10 ? 8 : 1;      // warps of a block
-   const int64_t most = p.kind == 20 ? 16 : (int64_t)sms * std::min(2, std::max(1, 512 / p.threads));
    const int64_t want = (rows + rows_at_once - 1) / rows_at_once;
-   p.blocks = (int)std::max<int64_t>(1, std::min(want, most));
+   p.blocks = (int)std::max<int64_t>(1, std::min(want, p.kind == 20 ? 16 : (int64_t)sms * per_sm));
    return p;
 }
 
@@ -835,13 +847,11 @@ template <class T, bool VEC> static int grad_of(GradArgs &a, const GradPlan &p, 
    constexpr bool WIDE = sizeof(T) == 8;
    a.group = 32;
    if (p.kind == 1) return launch_grad<T, 1, false, VEC, true, 256>(a, p, stream);
-   if (p.kind == 2) return launch_grad<T, 2, false, VEC, !WIDE, 256>(a, p, stream);
    if constexpr (VEC) {
       const int per_sm = (p.blocks + sms - 1) / sms;
-      const int64_t stage = a.n * (int64_t)sizeof(T) * (a.res.p != nullptr ? 3 : 2);
-      const int stages = (int)std::min<int64_t>(RING_MAX, (225 * 1024 / per_sm - 2048) / stage);
+      const int operands = a.res.p != nullptr ? 3 : 2, stages = grad_stages(a.n, sizeof(T), operands, per_sm);
       if (stages >= 2) {
-         const size_t smem = (size_t)(stages * stage);
+         const size_t smem = (size_t)(stages * operands * a.n * (int64_t)sizeof(T));
          if (p.kind == 11) return launch_grad_ring<T, 1>(a, p, stages, smem, stream);
          if (p.kind == 12) return launch_grad_ring<T, 2>(a, p, stages, smem, stream);
          if constexpr (!WIDE) return launch_grad_ring<T, 4>(a, p, stages, smem, stream);
