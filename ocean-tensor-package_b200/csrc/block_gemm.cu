@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(256) gemm_plain(const __grid_constant__ GemmAr
 constexpr int BM = 128;
 constexpr int TILE_P = BM * B8_BLOCK;                     // bytes of a stage's 128 rows
 
+constexpr int MAX_SPLITS = 8;                             // blocks of a cluster that share a tile: its portable size
 constexpr int AHEAD = 8;                                  // places for depth blocks' scales
 
 // PAIR: two blocks share a tile of 256 rows, each holds half of either operand's rows; the columns' half travels once
@@ -393,11 +394,17 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
       int tp, tq; place(first, tp, tq);
       const uint32_t part = tc::smem_u32(ring);
       const int cols = min(BN, (int)(a.q.rows - (int64_t)tq * BN));
-      for (int e = rank * S::threads + threadIdx.x; e < cols * BM; e += splits * S::threads) {
-         float v = 0;
-         for (int r = 0; r < splits; r++) v += tc::peer_load(part + 4 * e, r);
-         const int64_t p = (int64_t)tp * BM + (e & (BM - 1)), q = (int64_t)tq * BN + (e >> 7);
-         if (p < a.p.rows) store_c(a, p, q, v);
+      // four rows of a column at a time, all blocks' parts under way before the first is added
+      for (int e = rank * S::threads + threadIdx.x; e < cols * (BM / 4); e += splits * S::threads) {
+         float4 x[MAX_SPLITS];
+#pragma unroll
+         for (int r = 0; r < MAX_SPLITS; r++) if (r < splits) x[r] = tc::peer_load(part + 16 * e, r);
+         float v[4] = { x[0].x, x[0].y, x[0].z, x[0].w };
+#pragma unroll
+         for (int r = 1; r < MAX_SPLITS; r++) if (r < splits) { v[0] += x[r].x; v[1] += x[r].y; v[2] += x[r].z; v[3] += x[r].w; }
+         const int64_t p = (int64_t)tp * BM + (e & (BM / 4 - 1)) * 4, q = (int64_t)tq * BN + e / (BM / 4);
+#pragma unroll
+         for (int k = 0; k < 4; k++) if (p + k < a.p.rows) store_c(a, p + k, q, v[k]);
       }
    }
    if (PAIR || SPLIT) tc::cluster_sync();                 // no block leaves while another reads it or signals to it
@@ -497,14 +504,20 @@ static int gemm(GemmArgs &a, cudaStream_t stream)
    const int64_t ptiles = (a.p.rows + BM - 1) / BM;
    int bn = 256;
    if (a.q.rows <= 16) bn = 16; else if (a.q.rows <= 32) bn = 32; else if (a.q.rows <= 64) bn = 64; else if (a.q.rows <= 128) bn = 128;
-   else if (ptiles * ((a.q.rows + 255) / 256) < dev.sms) bn = 128;
+   else {
+      // A tile of 256 x 256 takes a pair of SMs about 1.5 times as long as a tile of 128 x 128 takes one (0.55 and 0.37 us
+      // a depth block); the fewer rounds decide (8192 rows by 512 tokens: 38 and 49 us, by 256: 35 and 27 us).
+      const int64_t pairs = std::max(1, dev.sms / 2), big = (a.p.rows + 255) / 256 * ((a.q.rows + 255) / 256);
+      const int64_t small = ptiles * ((a.q.rows + 127) / 128);
+      if (2 * ((small + dev.sms - 1) / dev.sms) < 3 * ((big + pairs - 1) / pairs)) bn = 128;
+   }
    const int64_t qtiles = (a.q.rows + bn - 1) / bn, tiles = ptiles * qtiles, kblocks = (a.K + B8_BLOCK - 1) / B8_BLOCK;
    if (ptiles > 0x3FFFFFF / qtiles) SD_ERROR("block_gemm: matrix too large");
    // A tile is shared by up to eight blocks (the portable size of a cluster) while there is room on the GPU and two
    // depth blocks are left for each.
    int splits = 1;
    const int64_t room = (int64_t)dev.sms * (bn < 128 ? 2 : 1);
-   while (splits < 8 && tiles * splits * 2 <= room && kblocks >= 4 * splits) splits *= 2;
+   while (splits < MAX_SPLITS && tiles * splits * 2 <= room && kblocks >= 4 * splits) splits *= 2;
    switch (bn) {
       case 16:  return launch_width<16>(a, splits, dev.sms, stream);
       case 32:  return launch_width<32>(a, splits, dev.sms, stream);

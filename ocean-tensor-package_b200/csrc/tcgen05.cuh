@@ -170,10 +170,10 @@ __device__ __forceinline__ void cluster_sync()
    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ float peer_load(uint32_t addr, uint32_t rank)
+__device__ __forceinline__ float4 peer_load(uint32_t addr, uint32_t rank)
 {
-   float v;
-   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at_rank(addr, rank)) : "memory");
+   float4 v;
+   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at_rank(addr, rank)) : "memory");
    return v;
 }
 
