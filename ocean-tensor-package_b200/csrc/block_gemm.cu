@@ -6,16 +6,24 @@
 // each block of 128 the epilogue's warps read it, apply both scales and add it to sums in registers.  While they do,
 // the tensor core works on the next block into the other half of tensor memory.
 //
-// Tiles of 128 x BN.  The 128 side lies on tensor memory's lanes, a thread of the epilogue each, so that its scale is one
-// register; the BN side lies on the columns, where a scale for 128 rows is one number a block as well, and a scale for
-// every row is a vector from shared memory.  Many tokens: tokens on the lanes, weights (128 x 128 scales) on the
-// columns, BN 256 or 128.  Few tokens: weights on the lanes, the tokens on 16 to 128 columns, and where the tiles do not
+// The rows of a tile lie on tensor memory's lanes, a thread of the epilogue each, so that their scale is one register; its
+// columns have one number a block where 128 of them share a scale, and a vector in shared memory where each has its own.
+// Many tokens: tokens on the lanes, weights (128 x 128 scales) on the columns, tiles of 256 x 256 for a pair of blocks or
+// of 128 x 128 for one.  Few tokens: weights on the lanes, the tokens on 16 to 128 columns, and where the tiles do not
 // fill the GPU a cluster of blocks shares a tile, each with a part of the depth, and adds the parts up through
 // distributed shared memory in the order of the blocks.
 //
+// Measured (K = 8192, 8192 rows of weights, half results): 8192 tokens 484 us (2.27 PFLOP/s, 1.39 times the rate of the
+// 16-bit library product, 70 % of twice that rate; about 570 us in a long row of calls at the power limit), 1024 tokens
+// 70 us, 128 tokens 27 us, 64 tokens 18.3 us, 16 tokens 16.0 us (64 % of the copy rate), one token 15.2 us; 4096 x 4096 by
+// one token 7.9 us.  The tensor cores take 512 cycles for a block of a pair, 555 with the loads alone; the epilogue's
+// chain (tensor memory's latency, scales, sums) makes it about 870.  With a scale for every column (weight gradients,
+// 4096 x 2000 x 5000: 71 us) the columns' vector costs another multiplication a sum and a shared-memory read, 1280 cycles.
+// Tried and slower: 16 epilogue warps of 64 columns (619 us), scales fetched four blocks at a time (558 us), one block a
+// tile of 128 x 256 (556 us: its 48 KB a block exceed the 64 bytes a cycle that an SM takes in).
+//
 // Operands whose codes are not on 16-byte boundaries take a plain kernel (shared-memory tiles, 32-bit arithmetic).
 #include <cuda.h>
-#include <mutex>
 #include "block8.cuh"
 #include "tcgen05.cuh"
 

@@ -5,12 +5,17 @@
 //   solid_gpu_rms_norm_quantize   the same with y as 8-bit codes, one scale for 128 elements of a row
 //   solid_gpu_rms_norm_grad       g = dy w,  dh = r g - h r^3 mean(g h) (+ dres),  dw = sum over rows of dy h r
 //
-// All of it is bound by memory: a row is read once, held in registers while its sums are formed, and written once.
-// Sums are kept in 32 bits (double: 64) and y is formed from the unrounded h; h, y and dh are rounded once, to nearest
-// even.  A row belongs to a warp or half warp when it has at most 1024 elements, to a block of up to 1024 threads up to
-// 16384 elements (double: 8192), beyond that to a block that reads it twice.  Blocks stay resident, keep the weights in
-// registers and fetch the next row before they reduce the present one, so that loads are in flight across the
-// reduction's barrier.
+// All of it is bound by memory: a row is read once and written once.  Sums are kept in 32 bits (double: 64) and y is
+// formed from the unrounded h; h, y and dh are rounded once, to nearest even.  A row belongs to a warp or half a warp up
+// to 512 elements (gradient: 256), to a block up to 16384, beyond that to a block that reads it twice.  Rows on 16-byte
+// boundaries come through a ring in shared memory (norm_ring, grad_ring); others, and those too long for two places of a
+// ring, are fetched by the threads themselves (norm_rows, grad_rows).  A row at a time in registers with the next one
+// fetched ahead was the first form: its loads shared the registers with the sums, 62 % of the copy rate.
+//
+// Measured on halves, the copy's rate (6.57 TB/s) as 100 %: norm with residual of 8192 rows of 4096 45.2 us (90 %), with
+// 8-bit output of 4096 rows of 8192 46.2 us (78 %: the conversions want more warps than the loads), gradient with residual
+// of 4096 rows of 4096 30.5 us (67 %, 4.5 us of it the join of the weights' gradient, whose partial rows have to be
+// written and read), one row of 4096 2.1 us (a launch).
 #include <atomic>
 #include "block8.cuh"
 #include "tcgen05.cuh"
@@ -647,7 +652,7 @@ static bool whole(const RowMatrix &m, size_t elemsize, size_t align, int64_t row
    return m.p == nullptr || (m.s0 == (int64_t)elemsize && (uintptr_t)m.p % align == 0 && (rows == 1 || m.s1 % (int64_t)align == 0));
 }
 
-static int matrix_of(const solid_gpu_matrix *m, int64_t n, size_t elemsize, const char *what, const char *op, bool optional, RowMatrix *out)
+static int matrix_of(const solid_gpu_matrix *m, size_t elemsize, const char *what, const char *op, bool optional, RowMatrix *out)
 {
    if (m == nullptr || m->ptr == nullptr) {
       if (!optional) SD_ERROR("%s: missing matrix %s", op, what);
@@ -657,7 +662,6 @@ static int matrix_of(const solid_gpu_matrix *m, int64_t n, size_t elemsize, cons
    if ((uintptr_t)m->ptr % elemsize != 0 || m->stride0 % (ptrdiff_t)elemsize != 0 || m->stride1 % (ptrdiff_t)elemsize != 0)
       SD_ERROR("%s: matrix %s must be aligned to its element size", op, what);
    *out = { (char *)m->ptr, (int64_t)m->stride0, (int64_t)m->stride1 };
-   (void)n;
    return 0;
 }
 
@@ -739,7 +743,9 @@ static int norm_of(NormArgs &a, cudaStream_t stream)
                                              : launch_norm_ring<T, 4, QUANT>(a, p, threads, sms, stream);
       }
    }
-   if (n <= 2048) return launch_norm<T, 1, true, VEC, true, QUANT, 256>(a, round32(eights), sms, stream);
+   if constexpr (!VEC) {
+      if (n <= 2048) return launch_norm<T, 1, true, VEC, true, QUANT, 256>(a, round32(eights), sms, stream);
+   }
    if (n <= 8192) return launch_norm<T, 2, true, VEC, !WIDE, QUANT, 512>(a, round32((eights + 1) / 2), sms, stream);
    if constexpr (!WIDE) {
       if (n <= NORM_MAX) return launch_norm<T, 4, true, VEC, false, QUANT, 512>(a, round32((eights + 3) / 4), sms, stream);
@@ -781,8 +787,8 @@ static int fill_norm(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x
    if (check_norm(dtype, n, rows, eps, weight, op, &es) != 0) return -1;
    a->n = (int64_t)n; a->rows = (int64_t)rows; a->w = weight; a->eps = eps; a->group = 32;
    a->scale = nullptr; a->ss0 = a->ss1 = 0; a->format = 0;
-   if (matrix_of(x, a->n, es, "x", op, false, &a->x) != 0 || matrix_of(residual, a->n, es, "residual", op, true, &a->res) != 0 ||
-       matrix_of(h, a->n, es, "h", op, true, &a->h) != 0) return -1;
+   if (matrix_of(x, es, "x", op, false, &a->x) != 0 || matrix_of(residual, es, "residual", op, true, &a->res) != 0 ||
+       matrix_of(h, es, "h", op, true, &a->h) != 0) return -1;
    return 0;
 }
 
@@ -857,7 +863,7 @@ template <class T, bool VEC> static int grad_of(GradArgs &a, const GradPlan &p, 
          if constexpr (!WIDE) return launch_grad_ring<T, 4>(a, p, stages, smem, stream);
       }
    }
-   if (p.kind == 11) return launch_grad<T, 1, true, VEC, false, 256>(a, p, stream);
+   if constexpr (!VEC) { if (p.kind == 11) return launch_grad<T, 1, true, VEC, false, 256>(a, p, stream); }
    if (p.kind == 12) return launch_grad<T, 2, true, VEC, false, 512>(a, p, stream);
    if constexpr (!WIDE) return launch_grad<T, 4, true, VEC, false, 512>(a, p, stream);
    return 0;
@@ -894,7 +900,7 @@ extern "C" int solid_gpu_rms_norm(int dtype, size_t n, size_t rows, const solid_
 {
    sd::NormArgs a;
    if (sd::fill_norm(dtype, n, rows, x, residual, weight, eps, h, "rms_norm", &a) != 0) return -1;
-   if (sd::matrix_of(y, a.n, (size_t)solid_gpu_type_size[dtype], "y", "rms_norm", false, &a.y) != 0) return -1;
+   if (sd::matrix_of(y, (size_t)solid_gpu_type_size[dtype], "y", "rms_norm", false, &a.y) != 0) return -1;
    if (n == 0 || rows == 0) return 0;
    return sd::norm_any<false>(dtype, a, stream);
 }
@@ -936,8 +942,8 @@ extern "C" int solid_gpu_rms_norm_grad(int dtype, size_t n, size_t rows, const s
    const size_t ws = (size_t)solid_gpu_worktype_size[dtype];
    if ((uintptr_t)dweight % ws != 0 || (uintptr_t)buffer % ws != 0) SD_ERROR("%s: dweight and buffer must be aligned to their element size", op);
    a.n = (int64_t)n; a.rows = (int64_t)rows; a.w = weight; a.eps = eps; a.part = nullptr; a.group = 32;
-   if (sd::matrix_of(dy, a.n, es, "dy", op, false, &a.dy) != 0 || sd::matrix_of(h, a.n, es, "h", op, false, &a.h) != 0 ||
-       sd::matrix_of(dres, a.n, es, "dres", op, true, &a.res) != 0 || sd::matrix_of(dh, a.n, es, "dh", op, false, &a.dh) != 0) return -1;
+   if (sd::matrix_of(dy, es, "dy", op, false, &a.dy) != 0 || sd::matrix_of(h, es, "h", op, false, &a.h) != 0 ||
+       sd::matrix_of(dres, es, "dres", op, true, &a.res) != 0 || sd::matrix_of(dh, es, "dh", op, false, &a.dh) != 0) return -1;
    if (n == 0) return 0;
    if (rows == 0) {                                       // no row: the weights' gradient is zero
       if (dweight != nullptr) SD_CUDA_CHECK(cudaMemsetAsync(dweight, 0, n * ws, stream));
