@@ -195,3 +195,53 @@ def test_far_rows(gpu):
     ops.copy(q.codes, codes)
     b = ops.block_quantize(Tensor.from_numpy(half(rng, n, 70), "half"))
     assert np.array_equal(got(ops.block_gemm(ops.Blocks(codes, q.scales), b)), got(ops.block_gemm(q, b)))
+
+
+def test_operands_of_any_strides(gpu):
+    """Scales with the blocks' index running fastest, rows in reverse order, a residual that is the same for all rows,
+    weights with gaps: what plain copies of them give."""
+    rng = np.random.default_rng(12)
+    n, rows, m = 520, 70, 200
+    x, w = half(rng, n, rows), half(rng, n, m)
+    tx = Tensor.from_numpy(x, "half")
+    back = tx.slice(1, rows - 1, -1, -1)
+    assert back.size == [n, rows] and np.array_equal(got(back), x[:, ::-1])
+    one = Tensor.from_numpy(half(rng, n, 1), "half")
+    gaps = Tensor.from_numpy(half(rng, 2 * n), "half").slice(0, 0, 2 * n, 2)
+    y, h = ops.rms_norm(back, gaps, EPS, one)
+    want, wanth = ops.rms_norm(ops.clone(back), ops.clone(gaps), EPS, ops.clone(one.broadcast_to([n, rows])))
+    assert np.array_equal(got(y), got(want)) and np.array_equal(got(h), got(wanth))
+    q, qb = ops.block_quantize(ops.clone(back)), ops.block_quantize(back)
+    assert np.array_equal(q.codes.numpy(), qb.codes.numpy()) and np.array_equal(q.scales.numpy(), qb.scales.numpy())
+    qw = ops.block_quantize(Tensor.from_numpy(w, "half"), 128)
+    c = got(ops.block_gemm(qw, q))
+    turned = ops.Blocks(q.codes, ops.clone(q.scales.T).T, q.format)
+    assert turned.scales.strides != q.scales.strides
+    assert np.array_equal(got(ops.block_gemm(qw, turned)), c)
+    # rows of the codes in reverse order: no tensor map takes them, the plain kernel does (other order of the same sums)
+    codes = ops.clone(q.codes)
+    reverse = ops.Blocks(codes.slice(1, rows - 1, -1, -1), q.scales.slice(0, rows - 1, -1, -1), q.format)
+    a, b = (ref.decode(t.codes.numpy(), "e4m3") * ref.spread(t.scales.numpy().astype(np.float64), *t.codes.size, k) for t, k in ((qw, 128), (q, 1)))
+    assert np.all(np.abs(got(ops.block_gemm(qw, reverse))[:, ::-1] - a.T @ b) <= 2.0 ** -24 * 136 * (np.abs(a).T @ np.abs(b)) + 2.0 ** -11 * np.abs(a.T @ b) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 200, 600])
+def test_what_is_not_finite_stays_in_its_row(gpu, tokens):
+    """A token with an infinity and one with a NaN: their results are NaN, all others what they are without them; results
+    beyond the range of halves are infinite."""
+    rng = np.random.default_rng(tokens)
+    k, m = 512, 640
+    x, w = half(rng, k, tokens), half(rng, k, m)
+    qw = ops.block_quantize(Tensor.from_numpy(w, "half"), 128)
+    clean = got(ops.block_gemm(qw, ops.block_quantize(Tensor.from_numpy(x, "half")), "float"))
+    bad = sorted({0, tokens - 1})
+    x[7, bad[0]], x[300, bad[-1]] = np.inf, np.nan
+    c = got(ops.block_gemm(qw, ops.block_quantize(Tensor.from_numpy(x, "half")), "float"))
+    assert np.all(np.isnan(c[:, bad]))
+    good = [t for t in range(tokens) if t not in bad]
+    assert np.array_equal(c[:, good], clean[:, good])
+    y = got(ops.rms_norm(Tensor.from_numpy(x, "half")))
+    assert np.all(np.isnan(y[300, bad[-1]])) and np.all(np.isfinite(y[:, good]))
+    big = np.full((k, tokens), 3e4, np.float16)
+    ones = ops.block_quantize(Tensor.from_numpy(np.ones((k, m), np.float16), "half"), 128)
+    assert np.all(np.isposinf(got(ops.block_gemm(ones, ops.block_quantize(Tensor.from_numpy(big, "half"))))))
