@@ -22,7 +22,8 @@
 // Tried and slower: 16 epilogue warps of 64 columns (619 us), scales fetched four blocks at a time (558 us), one block a
 // tile of 128 x 256 (556 us: its 48 KB a block exceed the 64 bytes a cycle that an SM takes in).
 //
-// Operands whose codes are not on 16-byte boundaries take a plain kernel (shared-memory tiles, 32-bit arithmetic).
+// Operands whose codes are not on 16-byte boundaries take a plain kernel (shared-memory tiles, 32-bit arithmetic; 13 TFLOP/s
+// at 2048 x 2048 x 2048).
 #include <cuda.h>
 #include "block8.cuh"
 #include "tcgen05.cuh"
