@@ -473,7 +473,9 @@ def fill_at(t: Tensor, positions, value) -> Tensor:
 # ----------------------------------------------------------------------------
 # A matrix [n, rows] is column-major like every tensor: a row (a token) is n elements side by side, and dimension 0 is
 # the one that a norm or a block of 128 runs along.  Further dimensions count as rows.  Half, float and double; results
-# are rounded once, to nearest even, with subnormals (the copy family rounds as the reference's CPU code does).
+# are rounded once, to nearest even, with subnormals.  Operands of different types are widened to their common type, which
+# is the results' type too.  The copy family's conversion to half is never used here: it rounds as the reference's CPU code
+# does, and turns what is below 2^-15 into zero.
 class Blocks(NamedTuple):
     """8-bit floating-point codes with scales: element (i, row) stands for codes[i, row] * scales[row // block, i // 128].
 
@@ -526,12 +528,29 @@ def _row_operand(t: Tensor, dtype: str, size, device, what: str):
     return t, r[0], _lib.Matrix(t.ptr, t.strides[0], r[1])
 
 
-def _row_input(x: Tensor, what: str):
+def _layer_type(what: str, x: Tensor, *others) -> str:
+    """The common type of an operator's operands (None: absent).  Widening a half or a float is exact."""
     if x.dtype not in ("half", "float", "double"):
         raise TypeError("%s is not available for type %s" % (what, x.dtype))
+    dtype = x.dtype
+    for t in others:
+        if t is not None and t.dtype != dtype:
+            dtype = common_type(dtype, t.dtype)
+    if dtype not in ("half", "float", "double"):
+        raise TypeError("%s is not available for type %s" % (what, dtype))
+    return dtype
+
+
+def _takes(dst: Tensor | None, dtype: str, what: str):
+    """Refuses a tensor of halves for a result that has more bits: the copy to half would flush and round otherwise."""
+    if dst is not None and dst.dtype in ("half", "chalf") and dtype != "half":
+        raise TypeError("%s is of type %s and cannot go into a tensor of type %s" % (what, dtype, dst.dtype))
+
+
+def _row_input(x: Tensor, dtype: str, what: str):
     if not x.size:
         raise ValueError("%s needs at least one dimension" % what)
-    return _row_operand(x, x.dtype, x.size, x.storage.device, "the input")
+    return _row_operand(x, dtype, x.size, x.storage.device, "the input")
 
 
 def _view(storage, dtype: str, size, strides, offset: int = 0) -> Tensor:
@@ -553,7 +572,7 @@ def _new(storage, size, dtype: str):
 
 
 def _norm_weight(weight, x: Tensor):
-    """The weights as the kernels take them (contiguous, in the type of x) and their address."""
+    """The weights as the kernels take them (contiguous, in the type of x, which is the operands' common one) and their address."""
     if weight is None:
         return None, None
     if weight.size != x.size[:1]:
@@ -600,8 +619,11 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residua
     """Root-mean-square norm along dimension 0: y = x * weight / sqrt(mean(x^2) + eps).
 
     With a residual the sum h = x + residual is normalised (before it is rounded) and returned too: (y, h).  dst and h
-    say where y and h go; h may be the residual's own tensor, dst that of x."""
-    x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, "rms_norm")
+    say where y and h go; h may be the residual's own tensor, dst that of x.  y and h have the operands' common type:
+    halves beside float weights or a float residual give floats."""
+    dtype = _layer_type("rms_norm", x, weight, residual)
+    _takes(dst, dtype, "the norm")
+    x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, dtype, "rms_norm")
     out, my = _result(dst, x.size, x.dtype, x.storage)
     lib, stream = _here(x.storage.device)
     lib.rms_norm(x.dtype, x.size[0], rows, mx, mr, pw, eps, mh, my, stream)
@@ -609,9 +631,10 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6, residua
     return y if total is None else (y, _delivered(total, h))
 
 
-def _norm_operands(x, weight, residual, h, what):
+def _norm_operands(x, weight, residual, h, dtype, what):
     """What rms_norm and rms_norm_quantize share.  The tensors are returned beside their addresses to keep them alive."""
-    x, rows, mx = _row_input(x, what)
+    _takes(h, dtype, "the sum")
+    x, rows, mx = _row_input(x, dtype, what)
     w, pw = _norm_weight(weight, x)
     if residual is None:
         if h is not None:
@@ -660,7 +683,8 @@ def rms_norm_quantize(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6
                       format: str = "e4m3", h: Tensor | None = None):
     """rms_norm whose y is returned as Blocks, a scale for 128 elements of each row; with a residual (Blocks, h)."""
     _format(format)
-    x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, "rms_norm_quantize")
+    dtype = _layer_type("rms_norm_quantize", x, weight, residual)
+    x, rows, mx, res, mr, w, pw, total, mh = _norm_operands(x, weight, residual, h, dtype, "rms_norm_quantize")
     out, view = _empty_blocks(x.size[0], rows, 1, format, x.storage)
     lib, stream = _here(x.storage.device)
     lib.rms_norm_quantize(x.dtype, x.size[0], rows, mx, mr, pw, eps, mh, view, stream)
@@ -671,11 +695,14 @@ def rms_norm_grad(dy: Tensor, h: Tensor, weight: Tensor | None = None, eps: floa
                   dst: Tensor | None = None):
     """Gradient of rms_norm at h (the input, or x + residual): returns (dh, dweight).
 
-    dres, the gradient that reaches h past the norm, is added to dh.  dweight is in the work type (half: float)."""
-    h, rows, mh = _row_input(h, "rms_norm_grad")
+    dres, the gradient that reaches h past the norm, is added to dh.  dh has the operands' common type, dweight the work type
+    of that (half: float)."""
     if dy.size != h.size or (dres is not None and dres.size != h.size):
         raise ValueError("gradients have the size of h, %s" % h.size)
-    device, dtype, n = h.storage.device, h.dtype, h.size[0]
+    dtype = _layer_type("rms_norm_grad", h, dy, weight, dres)
+    _takes(dst, dtype, "the gradient")
+    h, rows, mh = _row_input(h, dtype, "rms_norm_grad")
+    device, n = h.storage.device, h.size[0]
     dy, _, mg = _row_operand(dy, dtype, h.size, device, "dy")
     w, pw = _norm_weight(weight, h)
     mr = None
@@ -698,7 +725,7 @@ def block_quantize(x: Tensor, block: int = 1, format: str = "e4m3") -> Blocks:
     _format(format)
     if block not in (1, 128):
         raise ValueError("a scale belongs to 1 or 128 rows")
-    x, rows, mx = _row_input(x, "block_quantize")
+    x, rows, mx = _row_input(x, _layer_type("block_quantize", x), "block_quantize")
     out, view = _empty_blocks(x.size[0], rows, block, format, x.storage)
     lib, stream = _here(x.storage.device)
     lib.block_quantize(x.dtype, x.size[0], rows, mx, view, stream)
