@@ -732,14 +732,22 @@ def block_quantize(x: Tensor, block: int = 1, format: str = "e4m3") -> Blocks:
     return out
 
 
-def block_gemm(a: Blocks, b: Blocks, dtype: str = "half", dst: Tensor | None = None) -> Tensor:
+def block_gemm(a: Blocks, b: Blocks, dtype: str | None = None, dst: Tensor | None = None) -> Tensor:
     """Product of 8-bit matrices with scales: c[m, n] = sum over k of a[k, m] b[k, n], half or float.
+
+    Without a dtype the result has the type of dst (float where that is neither half nor float), and is half without dst.
+    A float result for a tensor of halves is rounded once, by the product itself.
 
     A linear layer with weights W [K, M] and tokens X [K, N] (both Blocks): y = block_gemm(W, X).  Its gradients:
     dX = block_gemm(block_quantize(w.T, 128), block_quantize(dy)), and dW = block_gemm(block_quantize(x.T),
     block_quantize(dy.T), "float"), a matrix [K, M]."""
+    if dtype is None:
+        dtype = "half" if dst is None or dst.dtype in ("half", "chalf") else "float"
     if dtype not in ("half", "float"):
         raise TypeError("block_gemm gives half or float, not %s" % dtype)
+    if dst is not None and dst.dtype == "half":
+        dtype = "half"
+    _takes(dst, dtype, "the product")
     ka, va = _blocks_view(a, "a")
     kb, vb = _blocks_view(b, "b")
     k, m = ka.size

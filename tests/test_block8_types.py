@@ -36,3 +36,9 @@ def test_complex_operands(other):
                  lambda: ops.rms_norm_quantize(x, residual=host([4, 3], other)), lambda: ops.rms_norm_grad(host([4, 3], other), x)):
         with pytest.raises(TypeError, match="not available for type c"):
             call()
+
+
+def test_a_float_product_into_complex_halves():
+    codes = ops.Blocks(host([256, 4], "uint8"), host([4, 2], "float"))
+    with pytest.raises(TypeError, match="the product is of type float"):
+        ops.block_gemm(codes, codes, "float", dst=host([4, 4], "chalf"))

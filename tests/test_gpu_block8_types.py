@@ -115,3 +115,30 @@ def test_into_a_tensor_of_more_bits(gpu, dtype, into):
     a, b = ops.rms_norm(upload(x, dtype), None, EPS, upload(r, dtype), dst=wide, h=wideh)
     assert a is wide and b is wideh
     assert np.array_equal(got(a), got(y).astype(got(a).dtype)) and np.array_equal(got(b), got(h).astype(got(b).dtype))
+
+
+@pytest.mark.parametrize("m,n,k", [(7, 3, 40), (300, 200, 512), (640, 40, 1000)])
+@pytest.mark.parametrize("size", [1.0, 300.0, 2.0 ** -22])
+def test_product_follows_its_result(gpu, m, n, k, size):
+    """Without a type, dst says how many bits are kept; halves are rounded to nearest even from the 32-bit sums, subnormals
+    among them (size 2^-22), numbers above 65504 stay finite in a float or double (size 300)."""
+    rng = np.random.default_rng(m)
+    a = ops.block_quantize(upload((values(rng, k, m, "float") * np.float32(size)), "float"), 128)
+    b = ops.block_quantize(upload((values(rng, k, n, "float") * np.float32(size if size > 1 else 1)), "float"))
+    c32 = ops.block_gemm(a, b, "float").numpy()
+    with np.errstate(over="ignore"):
+        c16 = c32.astype(np.float16)                         # numpy rounds to nearest even with subnormals
+    if size > 1:
+        assert np.any(np.abs(c32) > 65504)
+    if size < 1:
+        assert np.any((np.abs(c32) < 2.0 ** -15) & (c16 != 0))
+    for into, dtype, want in (("float", None, c32), ("double", None, c32), ("float", "float", c32), ("double", "float", c32),
+                              ("half", None, c16), ("half", "half", c16), ("half", "float", c16), ("float", "half", c16)):
+        full = Tensor.from_numpy(np.full((m + 1, n), 7, {"half": np.float16, "float": np.float32, "double": np.float64}[into]), into)
+        for dst in (Tensor.empty([m, n], into), Tensor.empty([n, m], into).T, full.slice(0, 1, m + 1)):
+            c = ops.block_gemm(a, b, dtype, dst=dst)
+            assert c is dst and np.array_equal(got(c), want.astype(got(c).dtype))
+        assert np.all(got(full)[0] == 7)
+    out = Tensor(Tensor.empty([m, n], "half").storage, "half", [m, n], None, 0, True)
+    assert np.array_equal(got(ops.block_gemm(a, b, "float", dst=out)), c16)      # bytes in the other order
+    assert ops.block_gemm(a, b).dtype == "half" and np.array_equal(got(ops.block_gemm(a, b)), c16)
