@@ -698,25 +698,34 @@ static int launch_norm(NormArgs &a, int threads, int sms, cudaStream_t stream)
 // only disturbs (halves, n 4096 with residual: 45 us with 128 KB, 49 us with 190 KB); four rows a block spread over
 // enough blocks for the arithmetic, which with 8-bit output is twice as much (n 4096: 58 us with 512 threads an SM, 47 us
 // with 1024).
+constexpr int64_t RING_ROOM = 225 * 1024, RING_STATIC = 2048;       // of an SM's shared memory; barriers and sums of a block
 struct RingPlan { int per_sm, stages; size_t smem; };
 static RingPlan ring_plan(int64_t stage_bytes, int threads, int threads_per_sm)
 {
-   constexpr int64_t UNDER_WAY = 128 * 1024, ROOM = 225 * 1024;
+   constexpr int64_t UNDER_WAY = 128 * 1024, ROOM = RING_ROOM;
    RingPlan p;
    p.per_sm = (int)std::min<int64_t>(16, std::max<int64_t>(UNDER_WAY / (RING_MAX * stage_bytes), threads_per_sm / threads));
    p.per_sm = std::max(1, std::min(p.per_sm, 2048 / threads));
-   while (p.per_sm > 1 && 2 * stage_bytes > ROOM / p.per_sm - 2048) p.per_sm--;
-   p.stages = (int)std::max<int64_t>(2, std::min<int64_t>(RING_MAX, (p.per_sm > 1 ? UNDER_WAY : ROOM - 2048) / (p.per_sm * stage_bytes)));
+   while (p.per_sm > 1 && 2 * stage_bytes > ROOM / p.per_sm - RING_STATIC) p.per_sm--;
+   p.stages = (int)std::max<int64_t>(2, std::min<int64_t>(RING_MAX, (p.per_sm > 1 ? UNDER_WAY : ROOM - RING_STATIC) / (p.per_sm * stage_bytes)));
    p.smem = (size_t)(p.stages * stage_bytes);
-   if (2 * stage_bytes > ROOM - 2048) p.per_sm = 0;       // not even two rows: no ring
+   if (2 * stage_bytes > ROOM - RING_STATIC) p.per_sm = 0;       // not even two rows: no ring
    return p;
+}
+
+// The limit on a kernel's shared memory belongs to the kernel, for all host threads.  So every call sets the same one, the
+// most that a plan asks for: one of its own could be lowered by another thread's call between setting and launch.
+template <class K> static int allow_ring(K kernel)
+{
+   SD_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(RING_ROOM - RING_STATIC)));
+   return 0;
 }
 
 template <class T, int V, bool QUANT>
 static int launch_norm_ring(NormArgs &a, const RingPlan &p, int threads, int sms, cudaStream_t stream)
 {
    auto *kernel = norm_ring<T, V, QUANT, 512>;
-   SD_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem));
+   if (allow_ring(kernel) != 0) return -1;
    kernel<<<(unsigned)std::min<int64_t>(a.rows, (int64_t)p.per_sm * sms), threads, p.smem, stream>>>(a, p.stages);
    SD_LAUNCH_CHECK();
    return 0;
@@ -798,7 +807,7 @@ struct GradPlan { int kind, threads, blocks; };
 
 static int grad_stages(int64_t n, size_t elemsize, int operands, int per_sm)
 {
-   return (int)std::min<int64_t>(RING_MAX, (225 * 1024 / per_sm - 2048) / (n * (int64_t)elemsize * operands));
+   return (int)std::min<int64_t>(RING_MAX, (RING_ROOM / per_sm - RING_STATIC) / (n * (int64_t)elemsize * operands));
 }
 
 template <class T> static bool grad_vec(const GradArgs &a)
@@ -842,7 +851,7 @@ static int launch_grad(GradArgs &a, const GradPlan &p, cudaStream_t stream)
 template <class T, int V> static int launch_grad_ring(GradArgs &a, const GradPlan &p, int stages, size_t smem, cudaStream_t stream)
 {
    auto *kernel = grad_ring<T, V, 512>;
-   SD_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+   if (allow_ring(kernel) != 0) return -1;
    kernel<<<p.blocks, p.threads, smem, stream>>>(a, stages);
    SD_LAUNCH_CHECK();
    return 0;
