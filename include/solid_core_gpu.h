@@ -465,7 +465,7 @@ SOLID_API int solid_gpu_peer_sum_float(int world, int rank, void *const *buffers
 /*   rms_norm_quantize  the same, y as codes with one scale for 128 elements of a row (y->block 1)                     */
 /*   rms_norm_grad      from dy and h: dh = r (dy w) - h r^3 mean(dy w h) (+ dres, optional), r = 1 / sqrt(mean(h^2)   */
 /*                      + eps), and dweight = sum over the rows of dy h r: n elements of the work type (half: float),  */
-/*                      optional.  buffer: device memory of rms_norm_grad_buffer_size bytes                            */
+/*                      optional.  buffer: device memory of rms_norm_grad_buffer_size bytes, aligned to the work type  */
 /*   block_quantize     codes and scales of x: scale = max(largest magnitude / largest code, 2^-126) over 128 elements  */
 /*                      of dimension 0 by y->block rows, code = x / scale rounded to nearest even (in 32 bits)         */
 /*   block_gemm         c[m, n] = sum over k of a[k, m] * b[k, n], a of size [K, M], b [K, N], c half or float [M, N]  */

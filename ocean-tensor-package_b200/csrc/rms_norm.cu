@@ -878,13 +878,16 @@ template <class T, bool VEC> static int grad_of(GradArgs &a, const GradPlan &p, 
    return 0;
 }
 
+// Partial rows are stored 16 bytes at a time, so they start on the caller's buffer's first such boundary
+constexpr size_t BUFFER_ALIGN = 16;
+
 template <class T> static int grad_typed(GradArgs &a, void *dw, void *buffer, cudaStream_t stream)
 {
    using W = typename Real<T>::acc;
    DeviceInfo dev;
    if (current_device_info(&dev) != 0) return -1;
    const GradPlan p = grad_plan(a.n, a.rows, sizeof(T), dev.sms);
-   W *rowsums = (W *)buffer;                              // long rows only
+   W *rowsums = (W *)(((uintptr_t)buffer + BUFFER_ALIGN - 1) / BUFFER_ALIGN * BUFFER_ALIGN);     // long rows only
    W *part = p.kind == 20 ? rowsums + 2 * a.rows : rowsums;
    a.part = dw != nullptr ? part : nullptr;
    if (p.kind == 20) {
@@ -936,7 +939,7 @@ extern "C" int solid_gpu_rms_norm_grad_buffer_size(int dtype, size_t n, size_t r
    const int sms = solid_gpu_multiprocessor_count(device);
    if (sms < 1) return -1;
    const sd::GradPlan p = sd::grad_plan((int64_t)n, (int64_t)rows, es, sms);
-   *size = ((size_t)p.blocks * n + (p.kind == 20 ? 2 * rows : 0)) * (size_t)solid_gpu_worktype_size[dtype];
+   *size = ((size_t)p.blocks * n + (p.kind == 20 ? 2 * rows : 0)) * (size_t)solid_gpu_worktype_size[dtype] + sd::BUFFER_ALIGN;
    return 0;
 }
 

@@ -712,7 +712,7 @@ def rms_norm_grad(dy: Tensor, h: Tensor, weight: Tensor | None = None, eps: floa
     dweight, md = _new(h.storage, [n], "double" if dtype == "double" else "float")
     lib, stream = _here(device)
     # a buffer of its own for each call: calls on several streams and captured graphs share nothing
-    buf = h.storage.new_empty(lib.rms_norm_grad_buffer_size(dtype, n, rows, device.index) + 16)
+    buf = h.storage.new_empty(lib.rms_norm_grad_buffer_size(dtype, n, rows, device.index))
     lib.rms_norm_grad(dtype, n, rows, mg, mh, pw, eps, mr, mo, md.ptr, buf.data_ptr(), stream)
     return _delivered(out, dst), dweight
 
