@@ -362,6 +362,8 @@ __global__ void __launch_bounds__(512) norm_long(const __grid_constant__ NormArg
 // ---------------------------------------------------------------------------
 // gradient
 // ---------------------------------------------------------------------------
+// With u = h r, the normalised row:  dh = r (g - u mean(g u)).  Each factor is then of the size of one of the operands;
+// r^3 by itself would leave the range of 32 bits for rows above 1e13 or below 1e-13.
 template <class T, int V, bool BLOCK, bool VEC, bool PIPE, int MAXT>
 __global__ void __launch_bounds__(MAXT, BLOCK || sizeof(T) == 8 ? 1 : 3) grad_rows(const __grid_constant__ GradArgs a)
 {
@@ -420,17 +422,17 @@ __global__ void __launch_bounds__(MAXT, BLOCK || sizeof(T) == 8 ? 1 : 3) grad_ro
          for (int k = 0; k < warps; k++) { s += sums[odd][0][k]; p += sums[odd][1][k]; }
       }
       const W rr = (W)1 / sqrt(s / (W)a.n + (W)a.eps);
-      const W c = rr * rr * rr * (p * inv_n);
+      const W c = rr * (p * inv_n);
 #pragma unroll
       for (int v = 0; v < V; v++) {
          const int64_t i = chunk_first<VEC>(v, group, t);
          W d[8];
 #pragma unroll
          for (int j = 0; j < 8; j++) {
-            const W gv = to_acc(cg[v].e[j]), hv = to_acc(ch[v].e[j]);
-            d[j] = fma(rr, gv * to_acc(w[v].e[j]), -hv * c);
+            const W gv = to_acc(cg[v].e[j]), u = to_acc(ch[v].e[j]) * rr;
+            d[j] = rr * fma(-u, c, gv * to_acc(w[v].e[j]));
             if (has_res) d[j] += to_acc(cr[v].e[j]);
-            dw[v][j] = fma(gv, hv * rr, dw[v][j]);
+            dw[v][j] = fma(gv, u, dw[v][j]);
          }
          put<T, VEC>(a.dh, row, i, a.n, d);
       }
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(MAXT) grad_ring(const __grid_constant__ GradAr
       s = 0; p = 0;
       for (int k = 0; k < threads / 32; k++) { s += sums[it & 1][0][k]; p += sums[it & 1][1][k]; }
       const W rr = (W)1 / sqrt(s / (W)a.n + (W)a.eps);
-      const W c = rr * rr * rr * (p * inv_n);
+      const W c = rr * (p * inv_n);
 #pragma unroll
       for (int v = 0; v < V; v++) {                       // the row once more from shared memory: no registers between
          const int i = (v * threads + t) * 8;
@@ -531,9 +533,9 @@ __global__ void __launch_bounds__(MAXT) grad_ring(const __grid_constant__ GradAr
             W d[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-               const W gv = to_acc(g.e[j]), hv = to_acc(h.e[j]);
-               d[j] = fma(rr, gv * to_acc(w[v].e[j]), -hv * c);
-               dw[v][j] = fma(gv, hv * rr, dw[v][j]);
+               const W gv = to_acc(g.e[j]), u = to_acc(h.e[j]) * rr;
+               d[j] = rr * fma(-u, c, gv * to_acc(w[v].e[j]));
+               dw[v][j] = fma(gv, u, dw[v][j]);
             }
             if (has_res) {
                const Eight<T> r = load_eight<T>(place + 2 * bytes + i * sizeof(T));
@@ -582,7 +584,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) grad_join(const W *__restrict
    if (lane == 0 && c < n) dw[c] = s;
 }
 
-// Long rows: a first kernel forms each row's r and r^3 mean(g h), a second one walks the columns
+// Long rows: a first kernel forms each row's r and r mean(g h), a second one walks the columns
 template <class T>
 __global__ void __launch_bounds__(512) grad_long_sums(const __grid_constant__ GradArgs a, typename Real<T>::acc *rowsums)
 {
@@ -609,7 +611,7 @@ __global__ void __launch_bounds__(512) grad_long_sums(const __grid_constant__ Gr
       if (threadIdx.x == 0) {
          const W rr = (W)1 / sqrt(s / (W)a.n + (W)a.eps);
          rowsums[2 * row] = rr;
-         rowsums[2 * row + 1] = rr * rr * rr * (p / (W)a.n);
+         rowsums[2 * row + 1] = rr * (p / (W)a.n);
       }
    }
 }
@@ -631,10 +633,10 @@ __global__ void __launch_bounds__(256) grad_long_apply(const __grid_constant__ G
       W d[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-         const W gv = to_acc(g.e[j]), hv = to_acc(h.e[j]);
-         d[j] = fma(rr, gv * to_acc(w.e[j]), -hv * c);
+         const W gv = to_acc(g.e[j]), u = to_acc(h.e[j]) * rr;
+         d[j] = rr * fma(-u, c, gv * to_acc(w.e[j]));
          if (a.res.p != nullptr) d[j] += to_acc(r.e[j]);
-         dw[j] = fma(gv, hv * rr, dw[j]);
+         dw[j] = fma(gv, u, dw[j]);
       }
       put<T, false>(a.dh, row, i, a.n, d);
    }

@@ -1,10 +1,12 @@
-"""Where the 8-bit linear layer's C functions read and write: places that a caller's own allocator gives."""
+"""The 8-bit linear layer at the ends of what it accepts: places that a caller's own allocator gives, numbers near the ends
+of their type's range."""
 import numpy as np
 import pytest
 
+import block8_ref as ref
 from solid_b200 import Tensor, ops
 from solid_b200._lib import Matrix
-from test_gpu_block8 import EPS, got, upload, values
+from test_gpu_block8 import ACC, EPS, STEP, got, roundings, upload, values
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +30,18 @@ def test_scratch_at_any_element(gpu, dtype, n, rows):
         assert np.array_equal(got(dh), got(want)) and np.array_equal(dw.numpy(), wantw.numpy())
         around = arena.cpu().numpy()
         assert np.all(around[:place] == 0xA5) and np.all(around[place + size:] == 0xA5)
+
+
+@pytest.mark.parametrize("dtype", ["float", "double"])
+@pytest.mark.parametrize("exponent", [50, -43])
+@pytest.mark.parametrize("n,rows,pad", [(64, 20, 0), (77, 9, 1), (1000, 30, 0), (1001, 5, 1), (4096, 400, 0), (8192, 20, 0), (16384, 2, 0), (17000, 4, 0)])
+def test_gradient_of_large_and_small_rows(gpu, dtype, exponent, n, rows, pad):
+    """Rows of 1e15 and of 1e-13 with eps 0: r^3 is beyond the range of 32 bits, the gradient is not.  The bounds are those
+    of ordinary rows: a power of two changes no rounding."""
+    rng = np.random.default_rng(n)
+    h = values(rng, n, rows, dtype) * (np.float32 if dtype == "float" else np.float64)(2.0 ** exponent)
+    dy, w = (values(rng, n, rows, dtype) * h.dtype.type(0.01)), values(rng, n, 1, dtype)[:, 0]
+    dh, dw = ops.rms_norm_grad(upload(dy, dtype, pad), upload(h, dtype, pad), upload(w, dtype), 0.0)
+    want, wantw, mag, magw = ref.rms_norm_grad(dy, h, w, 0.0, None)
+    assert np.all(np.abs(got(dh) - want) <= STEP[dtype] * np.abs(want) + ACC[dtype] * (2 * roundings(n) + 16) * mag)
+    assert np.all(np.abs(dw.numpy() - wantw) <= ACC[dtype] * (roundings(n) / 2 + rows + 16) * magw)
