@@ -24,6 +24,7 @@
 //
 // Operands whose codes are not on 16-byte boundaries take a plain kernel (shared-memory tiles, 32-bit arithmetic; 13 TFLOP/s
 // at 2048 x 2048 x 2048).
+#include <type_traits>
 #include <cuda.h>
 #include "block8.cuh"
 #include "tcgen05.cuh"
@@ -45,6 +46,25 @@ struct GemmArgs {
 __device__ __forceinline__ float scale_at(const Side &s, int64_t row, int64_t kb)
 {
    return row < s.rows ? __ldg(s.scale + (row >> s.shift) * s.s0 + kb * s.s1) : 0.0f;
+}
+// Scales p and q meet a sum x of 128 products of codes (zero, or 2^-32 to 2^39) as two factors, x * first * second: one and
+// their product, where that is an ordinary number or one of them is zero; else the larger one and the smaller.  x times the
+// larger leaves the range of 32 bits only where the result does, while a product out of range would make NaN of a sum of
+// zero, or lose bits of an ordinary result.
+__device__ __forceinline__ bool out_of_range(float v) { return ((__float_as_uint(v) & 0x7FFFFFFFu) - 0x00800000u) >= 0x7F000000u; }
+__device__ __forceinline__ bool in_turn(float p, float q) { return out_of_range(p * q) && p != 0.0f && q != 0.0f; }
+__device__ __forceinline__ float first_factor(float p, float q)  { return !in_turn(p, q) ? 1.0f : fabsf(p) > fabsf(q) ? p : q; }
+__device__ __forceinline__ float second_factor(float p, float q) { return !in_turn(p, q) ? p * q : fabsf(p) > fabsf(q) ? q : p; }
+// A row's scale that meets the sum before the column's: what lies outside 2^-90 to 2^88 gives a part of its exponent away,
+// so that x times the rest keeps its bits and stays finite; the column's scale takes that, and where it leaves the range
+// so does the result.
+__device__ __forceinline__ bool far_scale(float p) { return (__float_as_uint(p) & 0x7FFFFFFFu) - (37u << 23) > (178u << 23); }      // by the exponent's bits
+__device__ __forceinline__ float away(float p) { return fabsf(p) > 0x1p88f ? 0x1p40f : fabsf(p) < 0x1p-90f ? 0x1p-50f : 1.0f; }
+__device__ __forceinline__ float near_part(float p) { return fabsf(p) > 0x1p88f ? p * 0x1p-40f : fabsf(p) < 0x1p-90f ? p * 0x1p50f : p; }
+__device__ __forceinline__ uint32_t take_away(float q, float part)
+{
+   const float w = q * part;
+   return __float_as_uint(fabsf(w) == INFINITY && fabsf(q) < INFINITY ? copysignf(0x1.fffffep127f, q) : w);
 }
 __device__ __forceinline__ void store_c(const GemmArgs &a, int64_t p, int64_t q, float v)
 {
@@ -93,7 +113,10 @@ __global__ void __launch_bounds__(256) gemm_plain(const __grid_constant__ GemmAr
       for (int i = 0; i < 4; i++) {
          const float s = scale_at(a.p, p0 + tx + 16 * i, kb);
 #pragma unroll
-         for (int j = 0; j < 4; j++) acc[i][j] = fmaf(sum[i][j], s * scale_at(a.q, q0 + ty + 16 * j, kb), acc[i][j]);
+         for (int j = 0; j < 4; j++) {
+            const float t = scale_at(a.q, q0 + ty + 16 * j, kb);
+            acc[i][j] = fmaf(sum[i][j] * first_factor(s, t), second_factor(s, t), acc[i][j]);
+         }
       }
    }
 #pragma unroll
@@ -309,15 +332,8 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
 #pragma unroll
          for (int d = 0; d < AHEAD - 1; d++) fetch();
          uint64_t sum[CW / 2];                            // pairs of neighbouring columns
-#pragma unroll
-         for (int j = 0; j < CW / 2; j++) sum[j] = 0;
-         // Everything that the next block needs is under way before the present block's sums are done: its scales are
-         // read, its first columns are on their way from tensor memory.
-         auto scale_of = [&](int kb) {
-            const int slot = kb % AHEAD;
-            const float sp = scales[slot * SLOT + threadIdx.x];
-            return COLVEC ? sp : sp * scales[(AHEAD + slot) * SLOT + threadIdx.x];
-         };
+         auto row_scale = [&](int kb) { return scales[kb % AHEAD * SLOT + threadIdx.x]; };
+         auto col_scale = [&](int kb) { return scales[(AHEAD + kb % AHEAD) * SLOT + threadIdx.x]; };
          auto group_sync = [&] {
             if (group == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
             else            asm volatile("bar.sync 2, 128;" ::: "memory");
@@ -327,45 +343,93 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
             __syncwarp();
             tc::fence_after();
          };
-         constexpr int RUN = S::run, RUNS = CW / RUN;     // an even number: a block's first run is in v[0]
-         uint32_t v[2][RUN];
+#pragma unroll
+         for (int j = 0; j < CW / 2; j++) sum[j] = 0;
+         // The scales of a depth block: s for the whole warp's sums, unless it is `apart`, which is when a lane has scales for
+         // which the order of the multiplications matters.  Only rows and columns of the matrices count; others have zeros.
+         float s;
+         bool apart;
+         const bool inside = in_p && (COLVEC || in_q);
+         auto take_scales = [&](int kb) {
+            const float sp = row_scale(kb);
+            s = COLVEC ? sp : sp * col_scale(kb);
+            apart = __any_sync(0xFFFFFFFFu, inside && (COLVEC ? far_scale(sp) : out_of_range(s)));
+         };
+         auto next_scales = [&](int kb) {
+            tc::copies_wait<AHEAD - 3>();                 // the next block's scales, of every thread of the group
+            if (COLVEC) group_sync();                     // which is also past the place that is filled again
+            fetch();
+            take_scales(kb + 1 < kb1 ? kb + 1 : kb);
+         };
+         auto all_read = [&](int b) {                     // the next products may overwrite it
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) { if (PAIR) tc::bar_arrive_at(tempty_at + 8 * b); else tc::bar_arrive(tempty + 8 * b); }
+         };
          tc::copies_wait<AHEAD - 2>();
          if (COLVEC) group_sync();
-         float s = scale_of(kb0);
-         wait_sums(it);
-         tc::ld(from + (it & 1) * BN, v[0]);
-         for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int b = it & 1;
-            const float *cs = scales + (AHEAD + kb % AHEAD) * SLOT + group * 128;
-            const uint64_t s2 = tc::pair(__float_as_uint(s), __float_as_uint(s));
+         take_scales(kb0);
+         for (int kb = kb0; kb < kb1; ) {
+            if (apart) {                                  // one block by itself, with two factors for each sum
+               const float sp = row_scale(kb), sq = col_scale(kb);
+               const float *cs = scales + (AHEAD + kb % AHEAD) * SLOT + group * 128;
+               const float one = COLVEC ? near_part(sp) : first_factor(sp, sq), two = COLVEC ? away(sp) : second_factor(sp, sq);
+               wait_sums(it);
+               next_scales(kb);
 #pragma unroll
-            for (int c = 0; c < RUNS; c++) {
-               tc::ld_wait(v[c & 1]);
-               if (c + 1 < RUNS) tc::ld(from + b * BN + RUN * (c + 1), v[(c + 1) & 1]);
-               else {                                     // all read: the next products may overwrite it
-                  tc::fence_before();
-                  __syncwarp();
-                  if (lane == 0) { if (PAIR) tc::bar_arrive_at(tempty_at + 8 * b); else tc::bar_arrive(tempty + 8 * b); }
-                  if (kb + 1 < kb1) { wait_sums(it + 1); tc::ld(from + (b ^ 1) * BN, v[0]); }
-               }
-               if (c == 0) {
-                  tc::copies_wait<AHEAD - 3>();           // the next block's scales, of every thread of the group
-                  if (COLVEC) group_sync();               // which is also past the place that is filled again
-                  fetch();
-                  s = scale_of(kb + 1 < kb1 ? kb + 1 : kb);
-               }
+               for (int c = 0; c < CW; c += 8) {
+                  uint32_t x[8];
+                  tc::ld(from + (it & 1) * BN + c, x);
+                  tc::ld_wait(x);
+                  if (c + 8 == CW) all_read(it & 1);
 #pragma unroll
-               for (int j = 0; j < RUN; j += 4) {
-                  uint64_t x = tc::pair(v[c & 1][j], v[c & 1][j + 1]), y = tc::pair(v[c & 1][j + 2], v[c & 1][j + 3]);
-                  if (COLVEC) {
-                     const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(cs + RUN * c + j);
-                     x = tc::mul2(x, w.x); y = tc::mul2(y, w.y);
+                  for (int j = 0; j < 8; j += 2) {
+                     const uint64_t f = COLVEC ? tc::pair(take_away(cs[c + j], two), take_away(cs[c + j + 1], two)) : tc::pair(__float_as_uint(two), __float_as_uint(two));
+                     const uint64_t y = tc::mul2(tc::pair(x[j], x[j + 1]), tc::pair(__float_as_uint(one), __float_as_uint(one)));
+                     sum[(c + j) / 2] = tc::fma2(y, f, sum[(c + j) / 2]);
                   }
-                  const int k = (RUN * c + j) / 2;
-                  sum[k] = tc::fma2(x, s2, sum[k]);
-                  sum[k + 1] = tc::fma2(y, s2, sum[k + 1]);
                }
+               kb++; it++;
+               continue;
             }
+            // Everything that the next block needs is under way before the present block's sums are done: its scales are
+            // read, its first columns are on their way from tensor memory.
+            constexpr int RUN = S::run, RUNS = CW / RUN;  // an even number: a block's first run is in v[0]
+            uint32_t v[2][RUN];
+            bool more;
+            wait_sums(it);
+            tc::ld(from + (it & 1) * BN, v[0]);
+            do {
+               const int b = it & 1;
+               const float *cs = scales + (AHEAD + kb % AHEAD) * SLOT + group * 128;
+               const uint64_t s2 = tc::pair(__float_as_uint(s), __float_as_uint(s));
+#pragma unroll
+               for (int c = 0; c < RUNS; c++) {
+                  tc::ld_wait(v[c & 1]);
+                  if (c + 1 < RUNS) tc::ld(from + b * BN + RUN * (c + 1), v[(c + 1) & 1]);
+                  else {
+                     all_read(b);
+                     more = kb + 1 < kb1 && !apart;
+                     if (more) { wait_sums(it + 1); tc::ld(from + (b ^ 1) * BN, v[0]); }
+                  }
+                  if (c == 0) next_scales(kb);
+#pragma unroll
+                  for (int j = 0; j < RUN; j += 4) {
+                     uint64_t x = tc::pair(v[c & 1][j], v[c & 1][j + 1]), y = tc::pair(v[c & 1][j + 2], v[c & 1][j + 3]);
+                     const int k = (RUN * c + j) / 2;
+                     if (COLVEC) {
+                        const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(cs + RUN * c + j);
+                        x = tc::mul2(x, s2); y = tc::mul2(y, s2);
+                        sum[k] = tc::fma2(x, w.x, sum[k]);
+                        sum[k + 1] = tc::fma2(y, w.y, sum[k + 1]);
+                     } else {
+                        sum[k] = tc::fma2(x, s2, sum[k]);
+                        sum[k + 1] = tc::fma2(y, s2, sum[k + 1]);
+                     }
+                  }
+               }
+               kb++; it++;
+            } while (more);
          }
          float acc[CW];
 #pragma unroll

@@ -6,7 +6,7 @@ import pytest
 import block8_ref as ref
 from solid_b200 import Tensor, ops
 from solid_b200._lib import Matrix
-from test_gpu_block8 import ACC, EPS, STEP, got, roundings, upload, values
+from test_gpu_block8 import ACC, EPS, STEP, got, operand, roundings, upload, values
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,80 @@ def test_gradient_of_large_and_small_rows(gpu, dtype, exponent, n, rows, pad):
     want, wantw, mag, magw = ref.rms_norm_grad(dy, h, w, 0.0, None)
     assert np.all(np.abs(got(dh) - want) <= STEP[dtype] * np.abs(want) + ACC[dtype] * (2 * roundings(n) + 16) * mag)
     assert np.all(np.abs(dw.numpy() - wantw) <= ACC[dtype] * (roundings(n) / 2 + rows + 16) * magw)
+
+
+EXPONENTS = np.array([-149, -140, -126, -110, -91, -89, -60, -20, 0, 20, 60, 87, 89, 100, 119, 127])
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 1, 1000), (129, 3, 256), (512, 17, 640), (640, 64, 1500), (384, 100, 256), (128, 128, 128), (130, 129, 130),
+                                   (300, 520, 700), (1024, 2048, 512), (2500, 2300, 260)])
+@pytest.mark.parametrize("block_a,block_b,fa,fb", [(128, 1, "e4m3", "e4m3"), (1, 1, "e5m2", "e4m3"), (128, 128, "e5m2", "e5m2"), (1, 128, "e4m3", "e5m2")])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_scales_of_the_whole_range(gpu, m, n, k, block_a, block_b, fa, fb, aligned):
+    """Scales from the smallest float to the largest on either side: wherever the terms' magnitudes fit a float, the product
+    is as good as with ordinary scales, also where the two scales' own product is infinite or zero; zero codes give zero.
+
+    The bound is the ordinary one, and for what lands among the subnormals 2^-149 for each addition and 2^-149 for a term
+    that is rounded there."""
+    if not aligned and m * n > 100000:
+        pytest.skip("the plain kernel has no tiles of other sizes")
+    rng = np.random.default_rng(m + n + k)
+
+    def side(rows, block, fmt):
+        codes, scales, _ = operand(rng, k, rows, block, fmt)
+        codes[:, rng.integers(0, rows, rows // 8)] = 0
+        e = EXPONENTS[rng.integers(0, len(EXPONENTS), scales.shape)]
+        scales = np.ldexp(1 + rng.integers(0, 1 << 23, scales.shape) * 2.0 ** -23, e).astype(np.float32)
+        ld = (k + 15) // 16 * 16 + (0 if aligned else 1)
+        full = np.full((ld, rows), 0x7F, np.uint8)
+        full[:k] = codes
+        return codes, scales, ops.Blocks(Tensor.from_numpy(full, "uint8").slice(0, 0, k), Tensor.from_numpy(scales, "float"), fmt)
+
+    ca, sa, a = side(m, block_a, fa)
+    cb, sb, b = side(n, block_b, fb)
+    want, mag = ref.block_gemm(ca, sa, block_a, fa, cb, sb, block_b, fb)
+    c = got(ops.block_gemm(a, b, "float"))
+    fits = mag < 2.0 ** 127
+    assert np.any(fits)
+    tol = 2.0 ** -24 * (128 + 8 + k / 128) * mag + 2.0 ** -149 * (2 * (k // 128) + 4)
+    assert np.all(np.isfinite(c[fits])) and np.all(np.abs(c - want)[fits] <= tol[fits])
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 1, 1000), (129, 3, 256), (512, 17, 640), (640, 64, 1500), (384, 100, 256), (128, 128, 128), (130, 129, 130),
+                                   (300, 520, 700), (1024, 2048, 512), (2500, 2300, 260)])
+@pytest.mark.parametrize("block_a,block_b", [(128, 1), (1, 1), (128, 128), (1, 128)])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_scales_that_cancel(gpu, m, n, k, block_a, block_b, aligned):
+    """In each depth block one side's scales are as large as the other's are small, or both far from one: the results are
+    ordinary numbers, with the ordinary bound.  A row of zeros meets scales whose product is infinite."""
+    if not aligned and m * n > 100000:
+        pytest.skip("the plain kernel has no tiles of other sizes")
+    rng = np.random.default_rng(m + 2 * n + k)
+    nb = (k + 127) // 128
+    ea = EXPONENTS[rng.integers(0, len(EXPONENTS), nb)]
+    eb = np.clip(rng.choice([-30, 0, 30], nb) - ea, -146, 124)
+
+    def side(rows, block, e):
+        codes, scales, _ = operand(rng, k, rows, block, "e5m2")
+        codes[:, rng.integers(0, rows, rows // 8)] = 0
+        scales = np.ldexp(1 + rng.integers(0, 1 << 23, scales.shape) * 2.0 ** -23, np.minimum(e[None] + rng.integers(-3, 3, scales.shape), 127)).astype(np.float32)
+        scales[0, 0], codes[:128, :block] = 2.0 ** 127, 0    # a zero part under the largest scale
+        ld = (k + 15) // 16 * 16 + (0 if aligned else 1)
+        full = np.full((ld, rows), 0x7F, np.uint8)
+        full[:k] = codes
+        return codes, scales, ops.Blocks(Tensor.from_numpy(full, "uint8").slice(0, 0, k), Tensor.from_numpy(scales, "float"), "e5m2")
+
+    ca, sa, a = side(m, block_a, ea)
+    cb, sb, b = side(n, block_b, eb)
+    want, mag = ref.block_gemm(ca, sa, block_a, "e5m2", cb, sb, block_b, "e5m2")
+    assert np.all(mag < 2.0 ** 127)
+    for dtype in ("float", "half"):
+        c = got(ops.block_gemm(a, b, dtype))
+        tol = 2.0 ** -24 * (128 + 8 + k / 128) * mag + 2.0 ** -149 * (2 * nb + 4)
+        if dtype == "half":
+            tol = tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+            fits = np.abs(want) + tol < 65504
+            assert np.all(np.isinf(c[np.abs(want) - tol > 65536]))
+        else:
+            fits = np.full(want.shape, True)
+        assert np.all(np.abs(c - want)[fits] <= tol[fits])
