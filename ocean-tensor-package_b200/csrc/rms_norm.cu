@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(MAXT) norm_rows(const __grid_constant__ NormAr
 // ---------------------------------------------------------------------------
 // Whole rows on 16-byte boundaries come by bulk copies into a ring of `stages` rows (of each operand), so that the loads in
 // flight do not depend on registers or on the reduction's barrier: one thread refills a row's place after the barrier
-// of the next row, by which time every thread has finished with it.  A wait that runs out makes the thread's sums NaN,
-// and with them the row.
+// of the next row, by which time every thread has finished with it.  A wait that runs out makes the thread's elements NaN,
+// what is stored of x + residual among them, and through the sums the row's results.
 constexpr int RING_MAX = 4;
 
 struct Ring {
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(MAXT) norm_ring(const __grid_constant__ NormAr
 #pragma unroll
       for (int v = 0; v < V; v++) {
          const int i = (v * threads + t) * 8;
-         if (i < a.n) {
+         if (i < a.n && ring.ok) {
             const Eight<T> x = load_eight<T>(place + i * sizeof(T));
 #pragma unroll
             for (int j = 0; j < 8; j++) h[v][j] = to_acc(x.e[j]);
@@ -287,13 +287,13 @@ __global__ void __launch_bounds__(MAXT) norm_ring(const __grid_constant__ NormAr
                for (int j = 0; j < 8; j++) h[v][j] += to_acc(r.e[j]);
             }
          } else {
+            const W none = ring.ok ? (W)0 : (W)NAN;
 #pragma unroll
-            for (int j = 0; j < 8; j++) h[v][j] = 0;
+            for (int j = 0; j < 8; j++) h[v][j] = none;
          }
 #pragma unroll
          for (int j = 0; j < 8; j++) s = fma(h[v][j], h[v][j], s);
       }
-      if (!ring.ok) s = (W)NAN;
       s = row_sum<true>(s, threads, 0xFFFFFFFFu, sums[it & 1]);
       if (t == 0 && it > 0) load(it - 1 + stages);
       const W rr = (W)1 / sqrt(s / (W)a.n + (W)a.eps);
