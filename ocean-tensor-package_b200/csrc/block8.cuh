@@ -17,10 +17,10 @@ namespace sd {
 constexpr int B8_BLOCK = 128;                            // elements along dimension 0 that share a scale
 constexpr int B8_E4M3 = SOLID_GPU_E4M3, B8_E5M2 = SOLID_GPU_E5M2;
 
-// A caller's codes and scales: what every entry point asks of them
-static inline int check_blocks(const solid_gpu_blocks *b, const char *op, const char *what)
+// A caller's codes and scales: what every entry point asks of them.  Those of a matrix without elements may have no address.
+static inline int check_blocks(const solid_gpu_blocks *b, const char *op, const char *what, bool empty)
 {
-   if (b == nullptr || b->codes == nullptr || b->scales == nullptr) SD_ERROR("%s: missing codes or scales of %s", op, what);
+   if (b == nullptr || (!empty && (b->codes == nullptr || b->scales == nullptr))) SD_ERROR("%s: missing codes or scales of %s", op, what);
    if (b->format != SOLID_GPU_E4M3 && b->format != SOLID_GPU_E5M2) SD_ERROR("%s: unknown 8-bit format %d of %s", op, b->format, what);
    if (b->block != 1 && b->block != B8_BLOCK) SD_ERROR("%s: a scale of %s belongs to 1 or 128 rows, not to %d", op, what, b->block);
    if ((uintptr_t)b->scales % 4 != 0 || b->scale_stride0 % 4 != 0 || b->scale_stride1 % 4 != 0)

@@ -615,8 +615,8 @@ extern "C" int solid_gpu_block_gemm(int ctype, size_t M, size_t N, size_t K, con
    const char *op = "block_gemm";
    if (ctype != SD_HALF && ctype != SD_FLOAT) SD_ERROR("%s: the result's type must be half or float", op);
    if (M > ((size_t)1 << 40) || N > ((size_t)1 << 40) || K > ((size_t)1 << 40)) SD_ERROR("%s: matrix too large", op);
-   if (sd::check_blocks(a, op, "a") != 0 || sd::check_blocks(b, op, "b") != 0) return -1;
-   if (c == nullptr || c->ptr == nullptr) SD_ERROR("%s: missing matrix c", op);
+   if (sd::check_blocks(a, op, "a", M == 0 || K == 0) != 0 || sd::check_blocks(b, op, "b", N == 0 || K == 0) != 0) return -1;
+   if (c == nullptr || (c->ptr == nullptr && M != 0 && N != 0)) SD_ERROR("%s: missing matrix c", op);
    const ptrdiff_t es = solid_gpu_type_size[ctype];
    if ((uintptr_t)c->ptr % es != 0 || c->stride0 % es != 0 || c->stride1 % es != 0) SD_ERROR("%s: matrix c must be aligned to its element size", op);
    if (M == 0 || N == 0) return 0;

@@ -213,12 +213,13 @@ extern "C" int solid_gpu_block_quantize(int dtype, size_t n, size_t rows, const 
 {
    if (dtype != SD_HALF && dtype != SD_FLOAT && dtype != SD_DOUBLE) SD_ERROR("block_quantize: the type must be half, float or double");
    if (n > ((size_t)1 << 40) || rows > ((size_t)1 << 40)) SD_ERROR("block_quantize: matrix too large");
-   if (x == nullptr || x->ptr == nullptr) SD_ERROR("block_quantize: missing matrix x");
+   const bool empty = n == 0 || rows == 0;
+   if (x == nullptr || (x->ptr == nullptr && !empty)) SD_ERROR("block_quantize: missing matrix x");
    const ptrdiff_t es = solid_gpu_type_size[dtype];
    if ((uintptr_t)x->ptr % es != 0 || x->stride0 % es != 0 || x->stride1 % es != 0)
       SD_ERROR("block_quantize: matrix x must be aligned to its element size");
-   if (sd::check_blocks(y, "block_quantize", "y") != 0) return -1;
-   if (n == 0 || rows == 0) return 0;
+   if (sd::check_blocks(y, "block_quantize", "y", empty) != 0) return -1;
+   if (empty) return 0;
    sd::QuantArgs a = { (int64_t)n, (int64_t)rows, (const char *)x->ptr, (int64_t)x->stride0, (int64_t)x->stride1,
                        (char *)y->codes, (int64_t)y->ld, y->scales, (int64_t)y->scale_stride0 / 4, (int64_t)y->scale_stride1 / 4, y->format };
    if (dtype == SD_HALF)  return sd::quantize_typed<__half>(a, y->block, stream);

@@ -798,7 +798,8 @@ static int fill_norm(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x
    if (check_norm(dtype, n, rows, eps, weight, op, &es) != 0) return -1;
    a->n = (int64_t)n; a->rows = (int64_t)rows; a->w = weight; a->eps = eps; a->group = 32;
    a->scale = nullptr; a->ss0 = a->ss1 = 0; a->format = 0;
-   if (matrix_of(x, es, "x", op, false, &a->x) != 0 || matrix_of(residual, es, "residual", op, true, &a->res) != 0 ||
+   const bool empty = n == 0 || rows == 0;                // no element: no address needed
+   if (matrix_of(x, es, "x", op, empty, &a->x) != 0 || matrix_of(residual, es, "residual", op, true, &a->res) != 0 ||
        matrix_of(h, es, "h", op, true, &a->h) != 0) return -1;
    return 0;
 }
@@ -914,8 +915,9 @@ extern "C" int solid_gpu_rms_norm(int dtype, size_t n, size_t rows, const solid_
 {
    sd::NormArgs a;
    if (sd::fill_norm(dtype, n, rows, x, residual, weight, eps, h, "rms_norm", &a) != 0) return -1;
-   if (sd::matrix_of(y, (size_t)solid_gpu_type_size[dtype], "y", "rms_norm", false, &a.y) != 0) return -1;
-   if (n == 0 || rows == 0) return 0;
+   const bool empty = n == 0 || rows == 0;
+   if (sd::matrix_of(y, (size_t)solid_gpu_type_size[dtype], "y", "rms_norm", empty, &a.y) != 0) return -1;
+   if (empty) return 0;
    return sd::norm_any<false>(dtype, a, stream);
 }
 
@@ -925,9 +927,10 @@ extern "C" int solid_gpu_rms_norm_quantize(int dtype, size_t n, size_t rows, con
 {
    sd::NormArgs a;
    if (sd::fill_norm(dtype, n, rows, x, residual, weight, eps, h, "rms_norm_quantize", &a) != 0) return -1;
-   if (sd::check_blocks(y, "rms_norm_quantize", "y") != 0) return -1;
+   const bool empty = n == 0 || rows == 0;
+   if (sd::check_blocks(y, "rms_norm_quantize", "y", empty) != 0) return -1;
    if (y->block != 1) SD_ERROR("rms_norm_quantize: a scale belongs to one row (block 1)");
-   if (n == 0 || rows == 0) return 0;
+   if (empty) return 0;
    a.y = { (char *)y->codes, 1, (int64_t)y->ld };
    a.scale = y->scales; a.ss0 = (int64_t)y->scale_stride0 / 4; a.ss1 = (int64_t)y->scale_stride1 / 4; a.format = y->format;
    return sd::norm_any<true>(dtype, a, stream);
@@ -956,8 +959,9 @@ extern "C" int solid_gpu_rms_norm_grad(int dtype, size_t n, size_t rows, const s
    const size_t ws = (size_t)solid_gpu_worktype_size[dtype];
    if ((uintptr_t)dweight % ws != 0 || (uintptr_t)buffer % ws != 0) SD_ERROR("%s: dweight and buffer must be aligned to their element size", op);
    a.n = (int64_t)n; a.rows = (int64_t)rows; a.w = weight; a.eps = eps; a.part = nullptr; a.group = 32;
-   if (sd::matrix_of(dy, es, "dy", op, false, &a.dy) != 0 || sd::matrix_of(h, es, "h", op, false, &a.h) != 0 ||
-       sd::matrix_of(dres, es, "dres", op, true, &a.res) != 0 || sd::matrix_of(dh, es, "dh", op, false, &a.dh) != 0) return -1;
+   const bool empty = n == 0 || rows == 0;
+   if (sd::matrix_of(dy, es, "dy", op, empty, &a.dy) != 0 || sd::matrix_of(h, es, "h", op, empty, &a.h) != 0 ||
+       sd::matrix_of(dres, es, "dres", op, true, &a.res) != 0 || sd::matrix_of(dh, es, "dh", op, empty, &a.dh) != 0) return -1;
    if (n == 0) return 0;
    if (rows == 0) {                                       // no row: the weights' gradient is zero
       if (dweight != nullptr) SD_CUDA_CHECK(cudaMemsetAsync(dweight, 0, n * ws, stream));
