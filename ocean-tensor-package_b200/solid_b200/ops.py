@@ -673,8 +673,9 @@ def _blocks_view(b: Blocks, what: str):
     else:
         raise ValueError("%s: scales of size %s do not belong to codes of size %s" % (what, scales.size, codes.size))
     fmt = _format(b.format)
-    if n > 1 and codes.strides[0] != 1:
-        codes = clone(codes)
+    if n > 1 and codes.strides[0] != 1:                    # rows on 16-byte boundaries, for the tensor cores
+        ld = (n + 15) // 16 * 16
+        codes = copy(codes, _view(codes.storage.new_empty(ld * rows), "uint8", [n, rows], [1, ld]))
     return codes, _lib.BlocksView(codes.storage.data_ptr() + codes.offset, codes.strides[1],
                                   scales.storage.data_ptr() + scales.offset, scales.strides[0], scales.strides[1], block, fmt)
 

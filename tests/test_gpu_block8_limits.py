@@ -122,3 +122,15 @@ def test_scales_that_cancel(gpu, m, n, k, block_a, block_b, aligned):
         else:
             fits = np.full(want.shape, True)
         assert np.all(np.abs(c - want)[fits] <= tol[fits])
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 200, 1000), (300, 200, 1001), (640, 3, 515), (1024, 600, 270)])
+def test_turned_codes_reach_the_tensor_cores(gpu, m, n, k):
+    """Codes that are contiguous along the rows' dimension are laid out again with rows on 16-byte boundaries, whatever the
+    depth: the same bits as from codes that lay so from the start."""
+    rng = np.random.default_rng(k)
+    a, b = ops.block_quantize(upload(values(rng, k, m, "half"), "half"), 128), ops.block_quantize(upload(values(rng, k, n, "half"), "half"))
+    turned = [ops.Blocks(ops.clone(q.codes.T).T, q.scales, q.format) for q in (a, b)]
+    assert all(t.codes.strides[0] != 1 for t in turned)
+    assert all(ops._blocks_view(t, "a")[1].ld % 16 == 0 for t in turned)
+    assert np.array_equal(got(ops.block_gemm(*turned, "float")), got(ops.block_gemm(a, b, "float")))
