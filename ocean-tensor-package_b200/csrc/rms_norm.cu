@@ -757,8 +757,11 @@ static int norm_of(NormArgs &a, cudaStream_t stream)
    if constexpr (!VEC) {
       if (n <= 2048) return launch_norm<T, 1, true, VEC, true, QUANT, 256>(a, round32(eights), sms, stream);
    }
-   if (n <= 8192) return launch_norm<T, 2, true, VEC, !WIDE, QUANT, 512>(a, round32((eights + 1) / 2), sms, stream);
-   if constexpr (!WIDE) {
+   // Of whole rows, two fit the ring for all halves, for floats up to 8192 elements and for most doubles
+   if constexpr (!VEC || WIDE) {
+      if (n <= 8192) return launch_norm<T, 2, true, VEC, !WIDE, QUANT, 512>(a, round32((eights + 1) / 2), sms, stream);
+   }
+   if constexpr (!WIDE && (!VEC || sizeof(T) == 4)) {
       if (n <= NORM_MAX) return launch_norm<T, 4, true, VEC, false, QUANT, 512>(a, round32((eights + 3) / 4), sms, stream);
    }
    norm_long<T, QUANT><<<(unsigned)(a.rows < 4 * sms ? a.rows : 4 * sms), 512, 0, stream>>>(a);
@@ -876,9 +879,10 @@ template <class T, bool VEC> static int grad_of(GradArgs &a, const GradPlan &p, 
       }
    }
    if constexpr (!VEC) { if (p.kind == 11) return launch_grad<T, 1, true, VEC, false, 256>(a, p, stream); }
-   if (p.kind == 12) return launch_grad<T, 2, true, VEC, false, 512>(a, p, stream);
-   if constexpr (!WIDE) return launch_grad<T, 4, true, VEC, false, 512>(a, p, stream);
-   return 0;
+   // Of whole rows, two of three operands fit the ring for all halves and for floats up to 8192 elements
+   if constexpr (!VEC || WIDE) { if (p.kind == 12) return launch_grad<T, 2, true, VEC, false, 512>(a, p, stream); }
+   if constexpr (!WIDE && (!VEC || sizeof(T) == 4)) { if (p.kind == 14) return launch_grad<T, 4, true, VEC, false, 512>(a, p, stream); }
+   SD_ERROR("rms_norm_grad: no kernel for rows of %lld elements", (long long)a.n);
 }
 
 // Partial rows are stored 16 bytes at a time, so they start on the caller's buffer's first such boundary
