@@ -50,14 +50,17 @@ __device__ __forceinline__ float scale_at(const Side &s, int64_t row, int64_t kb
 // Scales p and q meet a sum x of 128 products of codes (zero, or 2^-32 to 2^39) as two factors, x * first * second: one and
 // their product, where that is an ordinary number or one of them is zero; else the larger one and the smaller.  x times the
 // larger leaves the range of 32 bits only where the result does, while a product out of range would make NaN of a sum of
-// zero, or lose bits of an ordinary result.
-__device__ __forceinline__ bool out_of_range(float v) { return ((__float_as_uint(v) & 0x7FFFFFFFu) - 0x00800000u) >= 0x7F000000u; }
+// zero, or lose bits of an ordinary result.  A half keeps its bits under any product but zero: x times one below 2^-126 is
+// below 2^-87, and wrong by 2^-110 at most.
+constexpr uint32_t LEAST_NORMAL = 0x00800000u, LEAST = 1u;         // as bits
+__device__ __forceinline__ bool out_of_range(float v, uint32_t least = LEAST_NORMAL) { return ((__float_as_uint(v) & 0x7FFFFFFFu) - least) >= 0x7F800000u - least; }
 __device__ __forceinline__ bool in_turn(float p, float q) { return out_of_range(p * q) && p != 0.0f && q != 0.0f; }
 __device__ __forceinline__ float first_factor(float p, float q)  { return !in_turn(p, q) ? 1.0f : fabsf(p) > fabsf(q) ? p : q; }
 __device__ __forceinline__ float second_factor(float p, float q) { return !in_turn(p, q) ? p * q : fabsf(p) > fabsf(q) ? q : p; }
 // A row's scale that meets the sum before the column's: what lies outside 2^-90 to 2^88 gives a part of its exponent away,
 // so that x times the rest keeps its bits and stays finite; the column's scale takes that, and where it leaves the range
-// so does the result.
+// so does the result.  A small one may stay whole where no column's scale is above one: what x times it loses among the
+// subnormals is then at most half the smallest one in the result too.  A batch's padding (zeros, scales of 2^-126) is that case.
 __device__ __forceinline__ bool far_scale(float p) { return (__float_as_uint(p) & 0x7FFFFFFFu) - (37u << 23) > (178u << 23); }      // by the exponent's bits
 __device__ __forceinline__ float away(float p) { return fabsf(p) > 0x1p88f ? 0x1p40f : fabsf(p) < 0x1p-90f ? 0x1p-50f : 1.0f; }
 __device__ __forceinline__ float near_part(float p) { return fabsf(p) > 0x1p88f ? p * 0x1p-40f : fabsf(p) < 0x1p-90f ? p * 0x1p50f : p; }
@@ -370,6 +373,15 @@ gemm_tiles(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CU
          if (COLVEC) group_sync();
          take_scales(kb0);
          for (int kb = kb0; kb < kb1; ) {
+            if (BN >= 128 && apart) {                     // small scales, a padded batch's: they may be no matter
+               if (COLVEC) {
+                  const float *cs = scales + (AHEAD + kb % AHEAD) * SLOT + group * 128;
+                  bool large = false;
+                  for (int c = lane; c < CW; c += 32) large |= fabsf(cs[c]) > 1.0f;
+                  large = __any_sync(0xFFFFFFFFu, large);
+                  apart = __any_sync(0xFFFFFFFFu, inside && far_scale(s) && (large || fabsf(s) > 1.0f));
+               } else if (a.half_out) apart = __any_sync(0xFFFFFFFFu, inside && out_of_range(s, LEAST));
+            }
             if (apart) {                                  // one block by itself, with two factors for each sum
                const float sp = row_scale(kb), sq = col_scale(kb);
                const float *cs = scales + (AHEAD + kb % AHEAD) * SLOT + group * 128;

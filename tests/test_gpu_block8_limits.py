@@ -134,3 +134,68 @@ def test_turned_codes_reach_the_tensor_cores(gpu, m, n, k):
     assert all(t.codes.strides[0] != 1 for t in turned)
     assert all(ops._blocks_view(t, "a")[1].ld % 16 == 0 for t in turned)
     assert np.array_equal(got(ops.block_gemm(*turned, "float")), got(ops.block_gemm(a, b, "float")))
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 1, 1000), (512, 17, 640), (130, 129, 130), (300, 520, 700), (1024, 2048, 512)])
+@pytest.mark.parametrize("block_a,block_b", [(128, 1), (1, 1), (1, 128)])
+@pytest.mark.parametrize("large", [False, True])
+def test_small_scales(gpu, m, n, k, block_a, block_b, large):
+    """One side's scales are those that a padded batch has beside ordinary ones (2^-126, and up to 2^-91), the other's at most
+    one, but for a single large one: floats keep their bits where they are ordinary, halves are as near as with any scales.
+    An infinite code keeps its infinity."""
+    rng = np.random.default_rng(m + 3 * n + k)
+
+    def side(rows, block, low, high):
+        codes, scales, _ = operand(rng, k, rows, block, "e5m2")
+        scales = np.ldexp(1 + rng.integers(0, 1 << 23, scales.shape) * 2.0 ** -23, rng.integers(low, high, scales.shape)).astype(np.float32)
+        return codes, scales
+
+    def blocks(codes, scales):                             # with padded rows: the plain kernel is not meant
+        full = np.full(((k + 15) // 16 * 16, codes.shape[1]), 0x7F, np.uint8)
+        full[:k] = codes
+        return ops.Blocks(Tensor.from_numpy(full, "uint8").slice(0, 0, k), Tensor.from_numpy(scales, "float"), "e5m2")
+
+    ca, sa = side(m, block_a, -20, 0)
+    cb, sb = side(n, block_b, -126, -90)
+    ordinary = rng.random(sb.shape) < 0.1
+    sb[ordinary] = 2.0 ** -rng.integers(1, 9, ordinary.sum())
+    sb[rng.random(sb.shape) < 0.3] = 2.0 ** -126
+    if large:
+        sa[-1, 0] = 2.0 ** 60
+    want, mag = ref.block_gemm(ca, sa, block_a, "e5m2", cb, sb, block_b, "e5m2")
+    a, b = blocks(ca, sa), blocks(cb, sb)
+    tol = 2.0 ** -24 * (128 + 8 + k / 128) * mag + 2.0 ** -149 * (2 * (k // 128) + 4)
+    assert np.all(np.abs(got(ops.block_gemm(a, b, "float")) - want) <= tol)
+    c = got(ops.block_gemm(a, b, "half"))
+    halves = tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + 2.0 ** -100
+    fits = np.abs(want) + halves < 65504
+    assert np.all(np.abs(c - want)[fits] <= halves[fits])
+
+    ca[5, 0], cb[5] = 0x7C, 0x3C                           # infinity times one in every column, whatever the scales
+    sb[:, 0] = 2.0 ** -126
+    a, b = blocks(ca, sa), blocks(cb, sb)
+    others, mag = ref.block_gemm(np.where(ca == 0x7C, 0, ca), sa, block_a, "e5m2", cb, sb, block_b, "e5m2")
+    for dtype in ("half", "float"):
+        c = got(ops.block_gemm(a, b, dtype))
+        fits = (np.abs(others) + 2.0 ** -24 * (128 + 8 + k / 128) * mag < 65504) | (dtype == "float")
+        assert np.all(c[0] == np.inf) and np.all(np.isfinite(c[1:][fits[1:]]))
+
+
+@pytest.mark.parametrize("dtype", ["half", "float"])
+def test_padded_batch(gpu, dtype):
+    """A batch whose last tokens are zeros: their products are zeros, the others' and the weights' gradient are those of the
+    batch without them, to the last bit."""
+    rng = np.random.default_rng(7)
+    k, m, used, n = 520, 700, 384, 768
+    w, x, dy = values(rng, k, m, "half"), values(rng, k, n, "half"), values(rng, m, n, "half")
+    x[:, used:], dy[:, used:] = 0, 0
+
+    def layer(tokens):
+        tx, ty = upload(x[:, :tokens], "half"), upload(dy[:, :tokens], "half")
+        y = ops.block_gemm(ops.block_quantize(upload(w, "half"), 128), ops.block_quantize(tx), dtype)
+        return got(y), got(ops.block_gemm(ops.block_quantize(tx.T), ops.block_quantize(ty.T), dtype))
+
+    y, dw = layer(n)
+    y0, dw0 = layer(used)
+    assert np.all(y[:, used:] == 0) and np.array_equal(y[:, :used], y0)
+    assert np.array_equal(dw, dw0)
