@@ -466,8 +466,8 @@ SOLID_API int solid_gpu_peer_sum_float(int world, int rank, void *const *buffers
 /*   rms_norm_grad      from dy and h: dh = r (dy w) - h r^3 mean(dy w h) (+ dres, optional), r = 1 / sqrt(mean(h^2)   */
 /*                      + eps), and dweight = sum over the rows of dy h r: n elements of the work type (half: float),  */
 /*                      optional.  buffer: device memory of rms_norm_grad_buffer_size bytes, aligned to the work type  */
-/*   block_quantize     codes and scales of x: scale = max(largest magnitude / largest code, 2^-126) over 128 elements  */
-/*                      of dimension 0 by y->block rows, code = x / scale rounded to nearest even (in 32 bits)         */
+/*   block_quantize     codes and scales of x, in 32 bits: scale = max(largest magnitude * (1 / largest code), 2^-126)  */
+/*                      over 128 elements of dimension 0 by y->block rows, code = x * (1 / scale), to nearest even     */
 /*   block_gemm         c[m, n] = sum over k of a[k, m] * b[k, n], a of size [K, M], b [K, N], c half or float [M, N]  */
 SOLID_API int solid_gpu_rms_norm(int dtype, size_t n, size_t rows, const solid_gpu_matrix *x, const solid_gpu_matrix *residual,
                                  const void *weight, double eps, const solid_gpu_matrix *h, const solid_gpu_matrix *y,

@@ -1,9 +1,10 @@
 // 8-bit floating-point codes with scales: the conversion shared by the norm with 8-bit output and by block_quantize.
 //
-//   scale = max(amax / top, 2^-126)      amax: largest magnitude of the block, top: largest finite value of the format
-//   code  = round(x * (1 / scale))       to nearest even, beyond top: top
+//   scale = max(amax * (1 / top), 2^-126)   amax: largest magnitude of the block, top: largest finite value of the format
+//   code  = round(x * (1 / scale))          to nearest even, beyond top: top
 //
-// in 32 bits.  The lower bound keeps 1 / scale finite, so that a block of zeros gets codes of zero.  A NaN in the block
+// in 32 bits, each quotient and product rounded: the scale is next to amax / top or the same (1.0e-7 apart at most), and a
+// value next to the middle of two codes may get either.  The lower bound keeps 1 / scale finite, so that a block of zeros gets codes of zero.  A NaN in the block
 // makes the scale and every code NaN; an infinity makes the scale infinite, its own code NaN and the others zero, so
 // that no product with the block is finite.
 #pragma once

@@ -13,12 +13,16 @@
 // fill the GPU a cluster of blocks shares a tile, each with a part of the depth, and adds the parts up through
 // distributed shared memory in the order of the blocks.
 //
-// Measured (K = 8192, 8192 rows of weights, half results): 8192 tokens 484 us (2.27 PFLOP/s, 1.39 times the rate of the
-// 16-bit library product, 70 % of twice that rate; about 570 us in a long row of calls at the power limit), 1024 tokens
-// 70 us, 128 tokens 27 us, 64 tokens 18.3 us, 16 tokens 16.0 us (64 % of the copy rate), one token 15.2 us; 4096 x 4096 by
-// one token 7.9 us.  The tensor cores take 512 cycles for a block of a pair, 555 with the loads alone; the epilogue's
-// chain (tensor memory's latency, scales, sums) makes it about 870.  With a scale for every column (weight gradients,
-// 4096 x 2000 x 5000: 71 us) the columns' vector costs another multiplication a sum and a shared-memory read, 1280 cycles.
+// Measured in a captured graph of a few calls (K = 8192, 8192 rows of weights, half results): 8192 tokens 487 us (2.26
+// PFLOP/s, 1.38 times the rate of the 16-bit library product, 69 % of twice that rate; in a long row of calls, at the power
+// limit, 583 to 598 us, 1.84 to 1.89 PFLOP/s, 56 to 58 %), 1024 tokens 71 us, 128 tokens 29 us, 64 tokens 20.5 us, 16 tokens
+// 17.3 us (59 % of the copy rate); 4096 x 4096 by one token 8.3 us.  The tensor cores take 512 cycles for a block of a pair,
+// 555 with the loads alone; the epilogue's chain (tensor memory's latency, scales, sums) makes it about 880.  With a scale
+// for every column (weight gradients, 4096 x 2000 x 5000: 76 us) the columns' vector costs another multiplication a sum
+// and a shared-memory read, 1300 cycles.  The look at the scales' range is 1 to 1.5 % of the large products.  Where it finds
+// scales for which the order of multiplication matters a depth block takes longer: half of 8192 tokens zeros, float
+// results, 523 us (480 without the look; half results, where it does not matter, 459 and 451); weight gradient with half of
+// its depth zeros 89 us (76).
 // Tried and slower: 16 epilogue warps of 64 columns (619 us), scales fetched four blocks at a time (558 us), one block a
 // tile of 128 x 256 (556 us: its 48 KB a block exceed the 64 bytes a cycle that an SM takes in).
 //

@@ -5,9 +5,11 @@
 // thread; where that is the rows' dimension (the codes of a transposed matrix) the codes turn in shared memory, one
 // byte each, so that both sides of the copy move whole lines.
 //
-// Measured: floats to e4m3 with square blocks, 8192 x 4096, 30.2 us (5.55 TB/s, 84 % of the copy rate); halves across to
-// e5m2, 4096 x 4096, 16.9 us (3.0 TB/s: a tile's load, two barriers and store are a chain that five blocks an SM overlap
-// only in part; with 128 x 128 tiles and three blocks it was 21.9 us).
+// Measured in a captured graph with inputs that rotate over more than the L2 cache: floats to e4m3 with square blocks, 8192 x
+// 4096, 32.1 us (5.2 TB/s, 80 % of the copy rate); halves of 4096 x 4096 with a scale for each row along 20.3 us, across
+// 19.4 us (38 and 40 %: a tile's load, two barriers and store are a chain that five blocks an SM overlap only in part; with
+// 128 x 128 tiles and three blocks 30 % slower), with square blocks 25.9 and 23.4 us (30 and 33 %); floats 17.4 to
+// 19.4 us (73 to 66 %), doubles 32.4 to 38.7 us (71 to 60 %); halves off 16-byte boundaries 31.5 us along, 24.8 across.
 #include "block8.cuh"
 
 namespace sd {

@@ -12,10 +12,14 @@
 // ring, are fetched by the threads themselves (norm_rows, grad_rows).  A row at a time in registers with the next one
 // fetched ahead was the first form: its loads shared the registers with the sums, 62 % of the copy rate.
 //
-// Measured on halves, the copy's rate (6.57 TB/s) as 100 %: norm with residual of 8192 rows of 4096 45.2 us (90 %), with
-// 8-bit output of 4096 rows of 8192 46.2 us (78 %: the conversions want more warps than the loads), gradient with residual
-// of 4096 rows of 4096 30.5 us (67 %, 4.5 us of it the join of the weights' gradient, whose partial rows have to be
-// written and read), one row of 4096 2.1 us (a launch).
+// Measured in a captured graph with inputs that rotate over more than the L2 cache, the copy's rate (6.57 TB/s) as 100 %,
+// halves with residual: norm of 8192 rows of 4096 48.6 us (84 %), with 8-bit output of 4096 rows of 8192 50.4 us (71 %: the
+// conversions want more warps than the loads), gradient of 4096 rows of 4096 33.2 us (61 %, 4.5 us of it the join of the
+// weights' gradient, whose partial rows have to be written and read), one row of 4096 2.4 us (a launch).
+// What the threads fetch themselves, 2^24 elements with residual: rows off 16-byte boundaries (4095 halves) norm 53.8 us
+// (38 %), 8-bit output 68.7 (26 %), gradient 71.4 (29 %); floats off them 75, 50 and 61 %.  The gradient of 16384 floats, for
+// which the ring has no room, holds 32 values of five arrays a thread and spills: 108 us (38 %); doubles of 8192 likewise,
+// 199 us (41 %).  Rows above 16384, read twice: norm of 32768 halves 75 us (27 %), floats 83 (49 %), gradient 127 (16 %) and 90.
 #include <atomic>
 #include "block8.cuh"
 #include "tcgen05.cuh"
@@ -823,9 +827,10 @@ template <class T> static bool grad_vec(const GradArgs &a)
           whole(a.dh, es, 16, a.rows) && (uintptr_t)a.w % 16 == 0;
 }
 
-// The number of partial rows follows from sizes alone, so that the buffer's size can be asked for beforehand and the
-// order of the sums does not depend on addresses.  Blocks of an SM: 1024 threads, as long as three operands' rows fit
-// the ring twice (halves, n 4096: 34 us with 512 threads, 30 us with 1024).
+// The number of partial rows follows from sizes alone, so that the buffer's size can be asked for beforehand.  (A row's own
+// sums are taken in another order where its elements come one by one, so the last bits do depend on alignment.)  Blocks
+// of an SM: 1024 threads, as long as three operands' rows fit the ring twice (halves, n 4096: 34 us with 512 threads, 30
+// us with 1024).
 static GradPlan grad_plan(int64_t n, int64_t rows, size_t elemsize, int sms)
 {
    const bool wide = elemsize == 8;

@@ -721,8 +721,8 @@ def rms_norm_grad(dy: Tensor, h: Tensor, weight: Tensor | None = None, eps: floa
 def block_quantize(x: Tensor, block: int = 1, format: str = "e4m3") -> Blocks:
     """8-bit codes of a matrix [n, rows] with a scale for 128 elements of dimension 0 by `block` (1 or 128) rows.
 
-    scale = max(largest magnitude / largest code, 2^-126); code = x / scale to nearest even.  Strides are free:
-    block_quantize(x.T) gives the codes of the transposed matrix."""
+    In 32 bits: scale = max(largest magnitude * (1 / largest code), 2^-126); code = x * (1 / scale) to nearest even.
+    Strides are free: block_quantize(x.T) gives the codes of the transposed matrix."""
     _format(format)
     if block not in (1, 128):
         raise ValueError("a scale belongs to 1 or 128 rows")
